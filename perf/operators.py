@@ -358,7 +358,7 @@ def run(s):
         mh.tree_verify_dev(_ptr(s.p), V, _ptr(s.q), V, B, N, V, _ptr(s.parent), _ptr(s.token), _ptr(s.u_accept), _ptr(s.u_sample),
                            _ptr(s.path), _ptr(s.n_acc), _ptr(s.next), st)
         return {"path": s.path, "n_acc": s.n_acc, "next": s.next}
-    ptrs = [[t.data_ptr() + 4 * i * t.stride(0) for i in range(case["blocks"])] for t in (*s.draft, *s.cache)]
+    ptrs = [[t[i].data_ptr() for i in range(case["blocks"])] for t in (*s.draft, *s.cache)]
     mh.tree_commit_dev(*ptrs, B, N, case["kd"], case["ctx"] + N, _ptr(s.pos), _ptr(s.path), _ptr(s.n_acc), _ptr(s.pos_out), st)
     return {"k": s.cache[0], "v": s.cache[1], "pos": s.pos_out}
 
