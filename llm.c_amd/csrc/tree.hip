@@ -423,8 +423,11 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeArgs a, int block
     if (t0 + 2 < t1) load(S2{}, t0 + 2);
 
     // Query rows r = 16 QT rb + 16 c + li, node r / G, head r % G; past the
-    // last row: that row again.  Scores in log2 units.
-    float q[QT][KS];
+    // last row: that row again.  Scores in log2 units.  The queries of nodes
+    // that are no token are whatever the workspace holds: their maximum starts
+    // at infinity, which no score passes, so that they have no say in when the
+    // wave's maxima move.
+    float q[QT][KS], m[QT];
     unsigned long long anc[QT];
     const float scale = a.scale * 1.4426950408889634f;
 #pragma unroll
@@ -439,15 +442,15 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeArgs a, int block
         const int n = min(rb * ROWS + 16 * c + li, rows - 1) / G;
         anc[c] = (unsigned long long)__shfl((unsigned)(node.anc >> 32), n) << 32 |
                  (unsigned)__shfl((unsigned)node.anc, n);
+        m[c] = live >> n & 1 ? kLow : INFINITY;
 #pragma unroll
         for (int s = 0; s < KS; ++s) q[c][s] *= scale;
     }
 
-    float m[QT], l[QT];
+    float l[QT];
     fx4 o[QT][DT];
 #pragma unroll
     for (int c = 0; c < QT; ++c) {
-        m[c] = kLow;
         l[c] = 0.0f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[c][d] = fx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -909,11 +912,15 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
     if (t0 + PW < t1) load(S1{}, t0 + PW);
 
     // The lane's query row (past the last one: that row again), scores in
-    // log2 units; qs undoes the row's factor.
+    // log2 units; qs undoes the row's factor.  Rows of nodes that are no token
+    // (whatever the workspace holds) have no say in the wave's decisions: they
+    // do not count for its range, and their maximum starts at infinity, which no
+    // score passes.
     const int r = (rb * RW + rw) * 32 + li, rq = min(r, rows - 1), qn = rq / G;
     const float *qrow = a.q + ((size_t)b * N + qn) * a.qd + (kvh * G + rq % G) * HD;
     const unsigned long long anc = (unsigned long long)__shfl((unsigned)(node.anc >> 32), qn) << 32 |
                                    (unsigned)__shfl((unsigned)node.anc, qn);
+    const bool token = live >> qn & 1;
     const float scale = a.scale * 1.4426950408889634f;
     Halves fq[KS];
     float qs;
@@ -936,14 +943,14 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
                 }
             }
         u = max(u, (unsigned)__shfl_xor(u, 32));
-        odd = __any(u >= __float_as_uint(kMostKey));
+        odd = __any(token && u >= __float_as_uint(kMostKey));
         const int e = min(11 - expo(u), 126);
 #pragma unroll
         for (int s = 0; s < KS; ++s) fq[s] = halve8(v[s], pow2(e));
         qs = pow2(-e);
     }
 
-    float m = kLow, l = 0.0f;
+    float m = token ? kLow : INFINITY, l = 0.0f;
     fx16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d)

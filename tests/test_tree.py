@@ -1097,3 +1097,40 @@ def test_many_sequences():
     finally:
         at.close()
     check_verify(*verify_case(3000, 4, 60, "tree", 34))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 4), (2, 16), (3, 40), (20, 12), (130, 3), (130, 8)], ids=lambda s: "x".join(map(str, s)))
+def test_attn_tree_bits_whatever_ran_before(shape, positions):
+    """Trees with unused nodes and nodes past the cache's end, after calls that
+    leave zero, ordinary, very large and NaN queries in the workspace: the
+    same bits each time, in every block size and projection form."""
+    B, N = shape
+    nh, nkv, hd, d, S = 8, 2, 16, 128, 300
+    print(f"[gpu-test] tree after other calls {shape}", flush=True)
+    pos = np.resize([S - 2, 200, 17], B)
+    x, w, kc, vc, pos, c, s, par = tree_case(B, N, d, nh, nkv, hd, S, pos, 130 + N, "holes", positions)
+    if N > 4:
+        par[:, N // 2] = -2
+    else:
+        par[:, 1] = -2
+    total = kc.shape[1]
+    dead = [ch is None for b in range(B) for ch in to.chains(par[b])]
+    assert any(dead) and not all(dead)
+    own = []
+    for scale in (1.0, 3000.0):
+        own.append(mh.Attn(d, nh, nkv, hd, total))
+        own[-1].load((scale * w["wq"]).astype(np.float32), w["wk"], w["wv"], w["wo"], w["rms"])
+        own[-1].set_rope(c, s)
+    every = np.full((B, N), -1, np.int32)
+    try:
+        first = None
+        for at, before in ((own[0], 0 * x), (own[0], x), (own[1], x), (own[0], np.full_like(x, np.nan))):
+            run_tree(before, w, kc, vc, np.zeros(B, np.int32), c, s, every, nh, nkv, hd, at=at)
+            got = run_tree(x, w, kc, vc, pos, c, s, par, nh, nkv, hd, at=own[0])
+            first = first or got
+            for u, v in zip(first, got):
+                assert np.array_equal(u, v)
+    finally:
+        for at in own:
+            at.close()
