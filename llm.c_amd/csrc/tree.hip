@@ -52,6 +52,9 @@ constexpr float kSlack = 16.0f;
 constexpr float kSplitLift = 7.0f, kSplitSlack = 15.0f;
 // Keys and queries from here on are left to float products.
 constexpr float kMostKey = 4096.0f;
+// And scores (log2 units) that the split could move by more than this: 2.6e-6 of
+// a probability.
+constexpr float kMostError = 0x1p-18f;
 constexpr float kLow = -3.0e38f;   // running maximum before the first score
 constexpr int kWaves = 4;
 constexpr int kMaxSplits = 128;
@@ -632,7 +635,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeArgs a, int block
 // float products: after a |K| or a query (in log2 units) of 2^12 or more, a
 // scaled K or V of 2^15 or more, an infinity (or, among the nodes, a NaN)
 // in V, or where in some dimension the largest |V| is more than 2^10 times the
-// largest of some four to eight positions (not all 0).
+// largest of some four to eight positions (not all 0).  And where the absolute
+// errors of K (2^-25 over its factor) and of Q (2^-36 of the row's maximum) can move
+// a score by more than kMostError: sum_d |q_d| 2^-25 / factor + HD max|q| 2^-36
+// max|K|, a bound that all errors of one sign would reach (a key dimension of
+// 4000 beside others of 0.003, queries of 333: 9e-5 in the output without the
+// rule, 8e-7 with it).
 //
 // A workgroup's four waves are RW blocks of 32 query rows times PW = 4 / RW tiles
 // of 32 positions; K and V of the PW tiles are split once by the workgroup and
@@ -702,6 +710,8 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
     // by dimension, and whether a key or value was out of range.
     constexpr int DV = 32 * DB;
     __shared__ unsigned sm_maxk[PW], sm_maxv[PW][DV], sm_most[PW][DV], sm_least[PW][DV];
+    __shared__ unsigned sm_mostk;   // the range's largest |K|
+    __shared__ float sm_qsum[4][32], sm_qmax[4][32];   // of the waves' rows: sum |q|, max |q|
     __shared__ int sm_odd;
     // Every eighth workgroup runs on one XCD: it takes an eighth of the
     // (sequence, kv head, split) triples, with all row blocks of each.
@@ -839,6 +849,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
     float sk[PW], sv[VI];             // factors of K by tile, of V by item
     float tk[PW], tv[VI];             // what is not below these is out of range
     float vmost[VI], vleast[VI];      // the item's largest |V| over the range, and the least but 0
+    float kmost = 0.0f;               // the largest |K| of the range
     bool out = false;                 // a key or value was out of range
 #pragma unroll
     for (int i = 0; i < VI; ++i) { vmost[i] = 0.0f; vleast[i] = INFINITY; }
@@ -851,7 +862,9 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
             int k;
             const int w = item(i, 64 * KS, k);
             if (64 * KS * PW % 256 && w >= PW) break;
-            out |= largest(kr[decltype(set)::value][i]) >= (PW > 1 && w ? tk[PW - 1] : tk[0]);
+            const float top = largest(kr[decltype(set)::value][i]);
+            kmost = fmaxf(kmost, top);
+            out |= top >= (PW > 1 && w ? tk[PW - 1] : tk[0]);
         }
 #pragma unroll
         for (int i = 0; i < VI; ++i) {
@@ -902,7 +915,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
         }
     };
     if (tid < PW) sm_maxk[tid] = 0;
-    if (tid == 0) sm_odd = 0;
+    if (tid == 0) sm_odd = 0, sm_mostk = 0;
     for (int i = tid; i < PW * DV; i += 256) {
         sm_maxv[i / DV][i % DV] = sm_most[i / DV][i % DV] = 0;
         sm_least[i / DV][i % DV] = ~0u;
@@ -928,6 +941,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
     {
         float v[KS][8];
         unsigned u = 0;
+        float sum = 0.0f;
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -940,9 +954,15 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
                     const float y = in ? x[e] * scale : 0.0f;
                     v[s][4 * i + e] = y;
                     u = max(u, __float_as_uint(y) & 0x7fffffffu);
+                    sum += fabsf(y);
                 }
             }
+        sum += __shfl_xor(sum, 32);
         u = max(u, (unsigned)__shfl_xor(u, 32));
+        if (lh == 0) {
+            sm_qsum[wave][li] = sum;
+            sm_qmax[wave][li] = __uint_as_float(u);
+        }
         odd = __any(token && u >= __float_as_uint(kMostKey));
         const int e = min(11 - expo(u), 126);
 #pragma unroll
@@ -1084,9 +1104,14 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
         atomicMax(&sm_most[w][k % DV], __float_as_uint(vmost[i]));
         atomicMin(&sm_least[w][k % DV], __float_as_uint(vleast[i]));
     }
+    kmost = wave_max(kmost);
+    if (lane == 0) atomicMax(&sm_mostk, __float_as_uint(kmost));
     if (out) sm_odd = 1;
     __syncthreads();
     {
+        const float ek = sm_qsum[wave][li] * pow2(max(-25 - factor(sm_maxk[pw], 0), -126));
+        const float eq = sm_qmax[wave][li] * (HD * 0x1p-36f) * __uint_as_float(sm_mostk);
+        odd |= __any(token && !(ek + eq <= kMostError));
         const unsigned most = sm_most[pw][lane % DV], least = sm_least[pw][lane % DV];
         odd |= sm_odd || __any(most && expo(most) - expo(least) > 10);
     }

@@ -1134,3 +1134,30 @@ def test_attn_tree_bits_whatever_ran_before(shape, positions):
     finally:
         for at in own:
             at.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [2, 8, 12, 40])
+def test_attn_tree_key_outliers(N):
+    """One key dimension near the largest that the split form takes, where the
+    queries are zero; the other keys small, the queries large: the attention
+    is the small ones'.  Scores are sums of 62 products around 1 (log2 units), whose
+    operands carry some roundings of 2^-24 each: sqrt(62) 3e-7 ln 2 = 2e-6 of
+    an exponential in the root mean square; the layer tolerance, on the rows of
+    attention alone."""
+    B, nh, nkv, hd, S = 2, 8, 2, 64, 150
+    x, w, kc, vc, pos, c, s, par = tree_case(B, N, 512, nh, nkv, hd, S, [140, 77], 140 + N, "tree", "many")
+    w["wo"] = np.eye(512, dtype=np.float32)
+    norm = np.sqrt((w["wq"].astype(np.float64) ** 2).sum(0).mean())
+    w["wq"] = (w["wq"] * (333.0 * 8 / 1.4427 / norm)).astype(np.float32)     # queries of 333 in log2 units
+    w["wk"] = (w["wk"] * (0.003 / np.sqrt((w["wk"].astype(np.float64) ** 2).sum(0).mean()))).astype(np.float32)
+    w["wq"][:, 62::64] = w["wq"][:, 63::64] = 0.0
+    kc[:, :S] = np.random.default_rng(N).standard_normal((B, S, nkv * hd)).astype(np.float32) * np.float32(0.003)
+    kc[:, :S:8, 62::64] = 4000.0
+    vc[:, :S] = np.random.default_rng(N + 1).standard_normal((B, S, nkv * hd)).astype(np.float32)
+    print(f"[gpu-test] key outliers N={N}", flush=True)
+    got = run_tree(x, w, kc, vc, pos, c, s, par, nh, nkv, hd)
+    y, _, _, live = to.attend(x, (w["wq"], w["wk"], w["wv"], w["wo"]), w["rms"], EPS, c, s, par, pos, kc, vc, nh, nkv, hd)
+    rel = orc.rel_l2((got[0].astype(np.float64) - x)[live], (y - x)[live])
+    print(f"[gpu-test]   rel-L2 {rel:.2e}", flush=True)
+    assert live.all() and rel <= 1e-5
