@@ -49,7 +49,10 @@ using split::kPairs;
 constexpr float kSlack = 16.0f;
 // The split kernel: m is kSplitLift below the maximum it was set from, and
 // moves when a score passes it by kSplitSlack.
-constexpr float kSplitLift = 7.0f, kSplitSlack = 15.0f;
+constexpr float kSplitLift = 12.0f, kSplitSlack = 15.0f;
+// Outputs whose dimensions are this much smaller (root mean square) than the
+// largest values there are left to float products.
+constexpr float kLeastOut = 0x1p-12f;
 // Keys and queries from here on are left to float products.
 constexpr float kMostKey = 4096.0f;
 // And scores (log2 units) that the split could move by more than this: 2.6e-6 of
@@ -627,10 +630,10 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeArgs a, int block
 //   Q   each row to a maximum in [2^11, 2^12);
 //   K   the range's first tile to [2^8, 2^9), the later ones by the same factor; its
 //       inverse and Q's join the exponential's fused multiply-add;
-//   P   e^(s - m) by 2^7, m lagging by 2^8 at most: up to 2^15;
+//   P   e^(s - m) by 2^12, m lagging by 2^3 at most: up to 2^15;
 //   V   each dimension of the first tile to [2^8, 2^9), the later ones likewise.
 // What is small beside those maxima keeps an absolute error: 2^-25 scaled, 2^-33 of
-// the first tile's largest |K| or of a dimension's largest |V| there, 2^-32 of a row's
+// the first tile's largest |K| or of a dimension's largest |V| there, 2^-37 of a row's
 // largest probability.  Where that might show, a wave takes its range again with
 // float products: after a |K| or a query (in log2 units) of 2^12 or more, a
 // scaled K or V of 2^15 or more, an infinity (or, among the nodes, a NaN)
@@ -640,7 +643,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeArgs a, int block
 // a score by more than kMostError: sum_d |q_d| 2^-25 / factor + HD max|q| 2^-36
 // max|K|, a bound that all errors of one sign would reach (a key dimension of
 // 4000 beside others of 0.003, queries of 333: 9e-5 in the output without the
-// rule, 8e-7 with it).
+// rule, 8e-7 with it).  And where a row's output is small beside the values that
+// it is made of, below kLeastOut of each dimension's largest |V| in the root mean
+// square: V's errors are 2^-21 of it there, P's of n positions sqrt(n) 2^-25 (a
+// position with values 1e-5 of the others' that takes all of the attention: up to
+// 6e-4 without the rule and P by 2^7).  Outputs that cancel to 1/sqrt(n) of
+// N(0, 1) values stay above it up to half a million positions.
 //
 // A workgroup's four waves are RW blocks of 32 query rows times PW = 4 / RW tiles
 // of 32 positions; K and V of the PW tiles are split once by the workgroup and
@@ -1114,6 +1122,18 @@ __global__ __launch_bounds__(256, 2) void tree_attn_split_kernel(TreeArgs a, int
         odd |= __any(token && !(ek + eq <= kMostError));
         const unsigned most = sm_most[pw][lane % DV], least = sm_least[pw][lane % DV];
         odd |= sm_odd || __any(most && expo(most) - expo(least) > 10);
+        const float g = most ? pow2(min(max(-le - expo(most), -126), 127)) : 0.0f;
+        float ss = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float y = o[d][e] * of_dim(g, d, e);
+                ss = fmaf(y, y, ss);
+            }
+        ss += __shfl_xor(ss, 32);
+        const float sum = (l + __shfl_xor(l, 32)) * kLeastOut;
+        odd |= __any(token && ss < __popcll(__ballot(most && lane < DV)) * (sum * sum));
     }
     if (odd) {
         // Float products (v_mfma_f32_32x32x2_f32), by each wave for itself,

@@ -1161,3 +1161,37 @@ def test_attn_tree_key_outliers(N):
     rel = orc.rel_l2((got[0].astype(np.float64) - x)[live], (y - x)[live])
     print(f"[gpu-test]   rel-L2 {rel:.2e}", flush=True)
     assert live.all() and rel <= 1e-5
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [22, 27, 32])
+@pytest.mark.parametrize("N", [2, 8, 12, 40])
+def test_attn_tree_small_values_of_a_likely_position(N, gap):
+    """A position that takes nearly all of the attention and has values 1e-5 of
+    the others', which are 2^gap less likely: the output is as small as its
+    values, and the others' probabilities and values must not blur it.  The
+    layer tolerance, on the rows of attention alone (W_O = 1e6, so that x
+    does not drown them)."""
+    B, nh, nkv, hd, S = 2, 8, 2, 64, 150
+    x, w, kc, vc, pos, c, s, par = tree_case(B, N, 512, nh, nkv, hd, S, [140, 77], 150 + N, "tree", "many")
+    rng = np.random.default_rng(gap)
+    w["wo"] = (1e6 * np.eye(512)).astype(np.float32)
+    x[:, :, 0] = 10.0
+    w["wq"][:, 62::64] = w["wq"][:, 63::64] = 0.0
+    w["wq"] *= np.float32(0.02)
+    w["wq"][0, 62::64] = 1.0                 # (a pair that RoPE hardly turns)
+    kc[:, :S] = rng.standard_normal((B, S, nkv * hd)).astype(np.float32)
+    vc[:, :S] = rng.standard_normal((B, S, nkv * hd)).astype(np.float32)
+    kc[:, :S, 62::64] = kc[:, :S, 63::64] = 0.0
+    w["wk"][:, 62::64] = w["wk"][:, 63::64] = 0.0
+    q = 10.0 * w["rms"][0] / np.sqrt((x.astype(np.float64) ** 2).mean())
+    kc[:, 7, 62::64] = gap * 8 / 1.4427 / q
+    vc[:, 7] *= np.float32(1e-5)
+    print(f"[gpu-test] small values N={N} gap {gap}", flush=True)
+    got = run_tree(x, w, kc, vc, pos, c, s, par, nh, nkv, hd)
+    y, _, _, live = to.attend(x, (w["wq"], w["wk"], w["wv"], w["wo"]), w["rms"], EPS, c, s, par, pos, kc, vc, nh, nkv, hd)
+    o = (y - x)[live]
+    assert live.all() and np.abs(o).max() < 1e3
+    rel = orc.rel_l2((got[0].astype(np.float64) - x)[live], o)
+    print(f"[gpu-test]   rel-L2 {rel:.2e}", flush=True)
+    assert rel <= 1e-5
