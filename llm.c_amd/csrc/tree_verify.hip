@@ -84,6 +84,14 @@ __device__ inline double wave_scan64(double v, int lane) {   // inclusive
     }
     return v;
 }
+__device__ inline double wave_back_scan64(double v, int lane) {   // of the lane and those above
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+        const double u = __shfl_down(v, s);
+        if (lane + s < 64) v += u;
+    }
+    return v;
+}
 
 // What is left of the target's distribution at one node: r(x) from p(x) and
 // q(x); with q null p(x), less the tokens that gone holds.
@@ -501,15 +509,17 @@ __global__ __launch_bounds__(THREADS) void tree_verify_kernel(VerifyArgs a, Veri
         }
     };
     // After a pass with the total t: w, and without q the sums after each
-    // further rejection.
+    // further rejection: the later children's, added up from the last one on
+    // (nothing is subtracted, so what is left of large and small tokens is as
+    // exact as its own sum, and no child's infinity outlives it).
     auto settle = [&](double t) {
         w = t;
         if (!has_q && i < N) {
             if (tid < 64) {
                 const bool in = tid < N && tid > 0 && sm.parent[tid] == cur && sm.first[tid];
                 const double v = in && sm.pt[tid] > 0.0f ? (double)sm.pt[tid] : 0.0;
-                const double sc = wave_scan64(v, tid);
-                sm.after[tid] = w + (__shfl(sc, 63) - sc);
+                const double later = __shfl_down(wave_back_scan64(v, tid), 1);
+                sm.after[tid] = w + (tid < 63 ? later : 0.0);
             }
             __syncthreads();
             w = sm.after[i];

@@ -1195,3 +1195,37 @@ def test_attn_tree_small_values_of_a_likely_position(N, gap):
     rel = orc.rel_l2((got[0].astype(np.float64) - x)[live], o)
     print(f"[gpu-test]   rel-L2 {rel:.2e}", flush=True)
     assert rel <= 1e-5
+
+
+@pytest.mark.gpu
+def test_tree_verify_looked_up_remainders():
+    """Looked-up drafts rejected against nearly all of the mass: what is left
+    is a sum of the tokens that are left, not a difference of larger sums.
+    Probabilities over 2^60, children that cover the whole support, an
+    infinite probability among them."""
+    print("[gpu-test] verify looked-up remainders", flush=True)
+    one = np.float32(1.0) - np.float32(2.0 ** -24)
+    star = lambda n: np.array([[-1] + [0] * n], np.int32)  # noqa: E731
+    p = np.zeros((1, 4, 4), np.float32)
+    p[0, 0] = [one, 1e-20, 2e-20, 0.0]
+    tok = np.array([[0, 0, 1, 2]], np.int32)
+    ua = np.array([[0, one, 0.9, 0.5]], np.float32)
+    path, n_acc, _ = check_verify(p, None, star(3), tok, ua, np.array([0.5], np.float32))
+    assert n_acc[0] == 1 and path[0, 1] == 3
+    rng = np.random.default_rng(17)
+    B = 200
+    for N, V, u in ((12, 11, 1.0), (40, 39, 1.0), (40, 200, 1.0), (64, 63, 0.0), (24, 5000, 0.0)):
+        p = np.zeros((B, N, V), np.float32)
+        p[:, 0] = 2.0 ** -rng.uniform(0, 60, (B, V))
+        p[:, 0] /= p[:, 0].sum(1, keepdims=True)
+        p[:, 1:] = 1.0 / V
+        tok = np.zeros((B, N), np.int32)
+        for b in range(B):
+            tok[b, 1:] = rng.permutation(V)[:N - 1] if b % 2 else p[b, 0].argsort()[::-1][:N - 1]
+        ua = np.full((B, N), u, np.float32) if u else np.maximum(rng.random((B, N)), 0.97).astype(np.float32)
+        par = np.repeat(star(N - 1), B, 0)
+        _, n_acc, nxt = check_verify(p, None, par, tok, ua, rng.random(B).astype(np.float32))
+        assert u < 1 or N <= V or (n_acc == 0).all()
+        # (the first child stays likely to be rejected, a later one is infinite)
+        p[:, 0, tok[np.arange(B), 3]] = np.inf
+        check_verify(p, None, par, tok, ua, rng.random(B).astype(np.float32))
