@@ -52,7 +52,8 @@ namespace moe {
 namespace {
 
 constexpr int kMaxSegs = 512;     // segments of a row
-constexpr int kListPairs = 18432; // pairs kept in LDS
+constexpr int kListPairs = 19000; // pairs kept in LDS
+constexpr int kListZero = kListPairs;     // behind them one that is zero, and one to write to that nobody reads
 constexpr int kQuads = 4;         // float4s of a row that a lane has in flight
 
 // Doubles across the wave.
@@ -92,7 +93,6 @@ __device__ inline double wave_back_scan64(double v, int lane) {   // of the lane
     }
     return v;
 }
-
 // What is left of the target's distribution at one node: r(x) from p(x) and
 // q(x); with q null p(x), less the tokens that gone holds.
 struct Left {
@@ -112,9 +112,14 @@ struct VerifySmem {
     int parent[64], token[64], gone[64], path[64];
     float u[64], pt[64], qt[64];
     bool first[64];            // no earlier child of the parent has the token
-    int ngone, listed, flag, claimed;   // listed: pairs asked room for (more than kListPairs: no list)
+    int ngone, listed, flag, claimed;   // listed: pairs asked room for (more than there is: no list)
     unsigned mask;
-    float2 list[kListPairs];
+    float2 list[kListPairs + 2];
+
+    // The list's room where the lanes' words for segs segments stand behind it
+    // (0: none do), and those words.
+    __device__ static int room(int segs) { return kListPairs - 16 * segs; }
+    __device__ unsigned short *lanes(int segs) { return reinterpret_cast<unsigned short *>(list + room(segs)); }
 };
 
 // Rows start at any float: four-byte aligned vector loads.
@@ -143,9 +148,11 @@ __device__ inline unsigned long long cload64(const unsigned long long *p) {
 // tokens again and leaves out what is not its own; V >= 4), so that the waits are
 // for the loads of a step and not for all.
 // LIST (segments of kQuads float4s per lane at most): pairs with something left
-// go to the list as well, if there is room; a segment's are together, where is
-// a matter of timing and of no other consequence.
-template <int WAVES, bool Q, bool LIST>
+// go to the list as well, if there is room; a segment's are together and in its
+// lanes' order, where is a matter of timing and of no other consequence.
+// LANES: where each lane's begin in its segment's and how many there are is kept
+// too, in a word 32 begin + number (all the list's segments are s0 .. s1 - 1).
+template <int WAVES, bool Q, bool LIST, bool LANES = false>
 __device__ void sum_segs(const Left &f, int V, int len, int s0, int s1, VerifySmem &sm) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int steps = len / (256 * kQuads);   // per segment
@@ -215,6 +222,7 @@ __device__ void sum_segs(const Left &f, int V, int len, int s0, int s1, VerifySm
                 const int u = __shfl_up(upto, d);
                 if (lane >= d) upto += u;
             }
+            if (LANES) sm.lanes(s1 - s0)[(s - s0) * 64 + lane] = (unsigned short)((upto - own) * 32 + own);
             const int all = __builtin_amdgcn_readlane(upto, 63);
             int at = 0;
             if (lane == 0) {
@@ -223,7 +231,7 @@ __device__ void sum_segs(const Left &f, int V, int len, int s0, int s1, VerifySm
                 sm.cnt[s] = all;
             }
             at = __builtin_amdgcn_readfirstlane(at);
-            if (at + all <= kListPairs) {
+            if (at + all <= sm.room(LANES ? s1 - s0 : 0)) {
                 at += upto - own;
 #pragma unroll
                 for (int e = 0; e < kQuads; ++e)
@@ -261,7 +269,7 @@ __device__ void sum_tiny(const Left &f, int V, VerifySmem &sm) {
     }
 }
 
-// The same from the list.
+// The same from the list, its pairs to the lanes in turn.
 template <int WAVES> __device__ void sum_list(double a, int s0, int s1, VerifySmem &sm) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     for (int s = s0 + wave; s < s1; s += WAVES) {
@@ -273,6 +281,53 @@ template <int WAVES> __device__ void sum_list(double a, int s0, int s1, VerifySm
         }
         t = wave_sum64(t);
         if (lane == 0) sm.seg[s] = t;
+    }
+}
+
+// The same, each lane taking what was its own, in order: the bits that sum_segs
+// gives (the tokens left out add 0).  Lanes keep only what still counts: the
+// first pass takes the longest lane's number of steps, up to 16, the later ones
+// some 7.  A wave's segments four at a time.
+template <int WAVES> __device__ void sum_lanes(double a, int s0, int s1, VerifySmem &sm) {
+    constexpr int G = 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned short *words = sm.lanes(s1 - s0) + lane;
+    for (int s = s0 + wave; s < s1; s += G * WAVES) {
+        int own[G], at[G], n[G], most = 0;
+        double t[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const int x = min(s + g * WAVES, s1 - 1), w = words[(x - s0) * 64];
+            own[g] = s + g * WAVES < s1 ? w & 31 : 0;
+            at[g] = sm.off[x] + (w >> 5);
+            n[g] = 0;
+            t[g] = 0.0;
+            most = max(most, own[g]);
+        }
+        for (int i = 0; __any(i < most); i += 2) {
+            float2 v[G][2];
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) v[g][u] = sm.list[i + u < own[g] ? at[g] + i + u : kListZero];
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const double r = left_of(v[g][u].x, v[g][u].y, a);
+                    t[g] += r;
+                    sm.list[i + u < own[g] ? at[g] + n[g] : kListZero + 1] = v[g][u];
+                    n[g] += r > 0.0;
+                }
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            if (s + g * WAVES >= s1) break;
+            unsigned short *w = words + (s + g * WAVES - s0) * 64;
+            *w = (unsigned short)((*w & ~31) | n[g]);
+            const double all = wave_sum64(t[g]);
+            if (lane == 0) sm.seg[s + g * WAVES] = all;
+        }
     }
 }
 
@@ -383,7 +438,8 @@ struct VerifyWords {
 // posts.  None waits without an end for another: a workgroup that sees no total
 // for some time leaves, a part that its own workgroup has not claimed when the
 // leader is done with its own falls to the leader, and so does a claimed one
-// that stays away (it is the same sum).
+// that stays away (it is the same sum, to the bit: from a list or from the rows
+// each lane adds its own tokens in order).
 template <int THREADS, bool TOGETHER>
 __global__ __launch_bounds__(THREADS) void tree_verify_kernel(VerifyArgs a, VerifyPlan pl) {
     constexpr int WAVES = THREADS / 64;
@@ -423,7 +479,10 @@ __global__ __launch_bounds__(THREADS) void tree_verify_kernel(VerifyArgs a, Veri
     bool summed = false, listed = false;
     double w = 1.0;
     Left f{a.p + row0 * a.ldp, has_q ? a.q + row0 * a.ldq : nullptr, 0.0, sm.gone, 0};
-    if (tid == 0) sm.path[0] = 0;
+    if (tid == 0) {
+        sm.path[0] = 0;
+        sm.list[kListZero] = make_float2(0.0f, 0.0f);
+    }
 
     // Lane i's node i, and the nodes whose token no earlier sibling has.
     const int lane = tid & 63;
@@ -503,7 +562,7 @@ __global__ __launch_bounds__(THREADS) void tree_verify_kernel(VerifyArgs a, Veri
             __syncthreads();
             if (tid == 0) sm.listed = 0;
             __syncthreads();
-            sum_segs<WAVES, true, true>(f, V, pl.len, s0, s1, sm);
+            sum_segs<WAVES, true, true, TOGETHER>(f, V, pl.len, s0, s1, sm);
         } else {
             sum_segs<WAVES, true, false>(f, V, pl.len, s0, s1, sm);
         }
@@ -563,7 +622,7 @@ __global__ __launch_bounds__(THREADS) void tree_verify_kernel(VerifyArgs a, Veri
         settle(total_of(segs, sm));
         while (i <= N && walk()) {
             __syncthreads();
-            const bool list = f.q && listed && sm.listed <= kListPairs;
+            const bool list = f.q && listed && sm.listed <= sm.room(TOGETHER ? p1 - p0 : 0);
             __syncthreads();    // (every thread has seen sm.listed)
             if (list) sum_list<WAVES>(f.a, 0, segs, sm);
             else      pass(0, segs, true);
@@ -589,9 +648,9 @@ __global__ __launch_bounds__(THREADS) void tree_verify_kernel(VerifyArgs a, Veri
                     const int k = __ffs(todo) - 1;
                     todo &= todo - 1;
                     __syncthreads();
-                    const bool list = own && f.q && listed && sm.listed <= kListPairs;
+                    const bool list = own && f.q && listed && sm.listed <= sm.room(TOGETHER ? p1 - p0 : 0);
                     __syncthreads();    // (every thread has seen sm.listed)
-                    if (list) sum_list<WAVES>(f.a, p0, p1, sm);
+                    if (list) sum_lanes<WAVES>(f.a, p0, p1, sm);
                     else      pass((int)((long long)segs * k / pl.parts), (int)((long long)segs * (k + 1) / pl.parts), own);
                 }
                 own = false;

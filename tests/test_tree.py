@@ -1229,3 +1229,128 @@ def test_tree_verify_looked_up_remainders():
         # (the first child stays likely to be rejected, a later one is infinite)
         p[:, 0, tok[np.arange(B), 3]] = np.inf
         check_verify(p, None, par, tok, ua, rng.random(B).astype(np.float32))
+
+
+def added_up(r, by_rank=None):
+    """A pass's total as the kernel adds it up, bit for bit: segments of 1024
+    tokens, of which lane l of a wave holds 256 e + 4 l + i (in this order of e
+    and i), the lanes' sums by a tree.  by_rank: the segment's tokens that this
+    marks in the lanes' order, every 64th to a lane (not what the kernel does)."""
+    def lanes(v):    # v[..., 64]
+        v = v.reshape(*v.shape[:-1], 4, 16)
+        for s in (1, 2, 4, 8):
+            v = v + np.concatenate((np.zeros_like(v[..., :s]), v[..., :-s]), -1)
+        v = v[..., 15]
+        return (v[..., 0] + v[..., 1]) + (v[..., 2] + v[..., 3])
+
+    V, segs = len(r), -(-len(r) // 1024)
+    full = np.zeros(segs * 1024)
+    full[:V] = r
+    mine = full.reshape(segs, 4, 64, 4).transpose(0, 2, 1, 3).reshape(segs, 64, 16)
+    if by_rank is not None:
+        mark = np.zeros(segs * 1024, bool)
+        mark[:V] = by_rank
+        mark = mark.reshape(segs, 4, 64, 4).transpose(0, 2, 1, 3).reshape(segs, 1024)
+        packed = np.zeros((segs, 1024))
+        for s in range(segs):
+            kept = mine[s].reshape(-1)[mark[s]]
+            packed[s, :len(kept)] = kept
+        mine = packed.reshape(segs, 16, 64).transpose(0, 2, 1)
+    t = np.zeros((segs, 64))
+    for k in range(16):
+        t = t + mine[..., k]
+    t = lanes(t)
+    c = -(-segs // 64)
+    t = np.concatenate((t, np.zeros(64 * c - segs))).reshape(64, c)
+    own = np.zeros(64)
+    for k in range(c):
+        own = own + t[:, k]
+    return lanes(own)
+
+
+def test_sum_orders_differ():
+    """The case below is one where the order decides (else it shows nothing)."""
+    p, q, par, tok, ua, us, accepted = tie_case()
+    p, q = p[0, 0], q[0, 0]
+    first = left_over(p, q, 1.0)
+    left = left_over(p, q, 1.0 + added_up(first))
+    assert added_up(left) != added_up(left, first > 0)
+    assert abs(added_up(left) - left.sum()) <= 1e-14 * left.sum()
+
+
+def left_over(p, q, a):
+    """max(p - a q, 0) in 64 bits, rounded once (a fused multiply-add)."""
+    from fractions import Fraction
+    return np.array([max(float(Fraction(float(x)) - Fraction(float(a)) * Fraction(float(y))), 0.0) for x, y in zip(p, q)])
+
+
+_TIE = []
+
+
+def tie_case():
+    """One sequence, a root with three children and a row of 65600 tokens: the
+    first two are rejected, the third's acceptance hangs on the last bits of the
+    sum of what they leave.  Its p and q are so small that they do not count in
+    the sums; p / q is a fraction as near to a + u W as 24-bit numbers come."""
+    from fractions import Fraction
+    if _TIE:
+        return _TIE[0]
+    V = 65600
+    for seed in range(40):
+        rng = np.random.default_rng(seed)
+        p = rng.random(V, dtype=np.float32) ** 8
+        p /= p.sum(dtype=np.float64)
+        q = (0.5 * (p + np.roll(p, 1))).astype(np.float32)
+        tok = np.array([0, 5, 70, 130], np.int32)
+        p[tok[1:3]] = 0.0
+        p[tok[3]] = q[tok[3]] = np.float32(2.0 ** -101)
+        w1 = added_up(left_over(p, q, 1.0))
+        a = 1.0 + w1
+        left = left_over(p, q, a)
+        rows, ranks = added_up(left), added_up(left, left_over(p, q, 1.0) > 0)
+        if rows == ranks:
+            continue
+        for _ in range(3000):
+            u = np.float32(rng.random() * 0.5 + 0.25)
+            X = Fraction(a) + Fraction(float(u)) * (Fraction(rows) + Fraction(ranks)) / 2
+            h, k, x = (0, 1), (1, 0), X      # convergents h / k of X
+            while True:
+                n = x.numerator // x.denominator
+                h, k = (h[1], n * h[1] + h[0]), (k[1], n * k[1] + k[0])
+                if h[1] >= 1 << 24 or k[1] >= 1 << 24:
+                    break
+                r = float(Fraction(h[1]) - Fraction(a) * k[1])
+                yes = [float(u) * k[1] * w < r for w in (rows, ranks)]
+                if yes[0] != yes[1] and k[1] >= 1 << 10:
+                    p[tok[3]], q[tok[3]] = np.float32(h[1] * 2.0 ** -123), np.float32(k[1] * 2.0 ** -123)
+                    N = 4
+                    P, Q = np.repeat(p[None, None], N, 1), np.repeat(q[None, None], N, 1)
+                    par = np.array([[-1, 0, 0, 0]], np.int32)
+                    ua = np.array([[0.0, 0.5, 0.5, u]], np.float32)
+                    _TIE.append((P, Q, par, tok[None].copy(), ua, np.array([0.37], np.float32), yes[0]))
+                    return _TIE[0]
+                if x == n:
+                    break
+                x = 1 / (x - n)
+    raise AssertionError("no such case")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B", [64, 30, 1])
+def test_tree_verify_one_order_of_sums(B):
+    """The passes over long rows are shared by a sequence's workgroups, which
+    add up a part from a list or, in another's place, from the rows: the same
+    order and the same bits by either way, so that equal sequences get equal
+    results however the workgroups happen to run."""
+    print(f"[gpu-test] verify order of sums B={B}", flush=True)
+    p, q, par, tok, ua, us, accepted = tie_case()
+    V = p.shape[2]
+    d = [dev(np.repeat(t, B, 0)) for t in (par, tok, ua, us)]
+    # (all sequences read the same rows: node 0's, and the third child's)
+    dp, dq = dev(np.repeat(p, B, 0)), dev(np.repeat(q, B, 0))
+    out = [mh.DeviceArray(sh, np.int32) for sh in ((B, 4), (B,), (B,))]
+    for _ in range(20):
+        mh.tree_verify_dev(dp.ptr, V, dq.ptr, V, B, 4, V, *[t.ptr for t in d + out])
+        path, n_acc, nxt = [o.to_host() for o in out]
+        assert (n_acc == int(accepted)).all(), n_acc
+        assert (path == path[0]).all() and (nxt == nxt[0]).all()
