@@ -1010,8 +1010,7 @@ int moe_hip_attn_tree_dev(MoeHipAttn *a, const float *x, float *y, int B, int N,
     t.wqkv_p = a->wqkv_p; t.wo_p = a->wo_p;
     t.wqkv_s = a->split_range[1] ? nullptr : a->wqkv_s;
     t.wo_s = a->split_range[3] ? nullptr : a->wo_s;
-    t.small_qkv = moe::split_small_sum(a->d, a->split_range[0]);
-    t.small_wo = moe::split_small_sum(qd, a->split_range[2]);
+    t.range = a->range;
     t.cos_t = a->cos_t; t.sin_t = a->sin_t;
     t.kc = const_cast<float *>(k_cache); t.vc = const_cast<float *>(v_cache); t.pos = pos;
     t.q = g_ws.aq.as<float>(); t.o = g_ws.ao.as<float>(); t.part = g_ws.apart.as<float>();

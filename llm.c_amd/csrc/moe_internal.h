@@ -270,9 +270,11 @@ struct TreeArgs : AttnArgs {
     const int *parent = nullptr;   // [rows]
     float *kd_out = nullptr, *vd_out = nullptr, *y = nullptr;
     // [wq | wk | wv] and wo as bf16 terms (launch_pack_split), null where a
-    // weight does not fit them; sums below small_* are not taken from them.
+    // weight does not fit them.  range [4]: their number ranges
+    // (launch_pack_split), read by each launch, so that a captured one computes
+    // with those of the weights that are loaded when it runs.
     const unsigned short *wqkv_s = nullptr, *wo_s = nullptr;
-    float small_qkv = 0.0f, small_wo = 0.0f;
+    const unsigned *range = nullptr;
     int *row_p = nullptr;          // [rows] workspace: RoPE position, -1: no token
     // Splits of a sequence's positions: partial maxima, sums and outputs
     // (TreePlan) in part when splits > 1.
@@ -298,11 +300,10 @@ TreePlan tree_plan(int seqs, int N, int nh, int nkv, int hd, int max_seq);
 // A K x N matrix as columns col0 .. of split weights (tree.hip); dst holds
 // split_weight_bytes(K, all columns), zero where no column or k is.
 // range [2], zero before the first: the bits of the largest |value|, and 1 if
-// one does not fit.  split_small_sum: TreeArgs::small_* for that largest.
+// one does not fit.
 size_t split_weight_bytes(int K, int N);
 hipError_t launch_pack_split(const float *src, unsigned short *dst, int K, int N, int col0,
                              unsigned *range, hipStream_t s);
-float split_small_sum(int K, unsigned most);
 hipError_t launch_attn_tree(const TreeArgs &a, hipStream_t s);
 
 // Verification of drafted tokens (tree_verify.hip).

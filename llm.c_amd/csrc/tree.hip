@@ -33,7 +33,6 @@
 #include "moe_internal.h"
 #include "moe_math.h"
 #include <algorithm>
-#include <cstring>
 
 namespace moe {
 namespace {
@@ -130,8 +129,9 @@ namespace {
 // Number range: the split holds an operand to 2^-134 at worst (its last
 // term is a bfloat16 subnormal), 24 bits from 2^-109 on.  Weights with a
 // nonzero value below that, or one of 2^127 and more, are not used in this form
-// at all (TreeArgs::wqkv_s null), so a sum over K products of weights up to w is
-// off by at most K w 2^-134 from it: a sum below a.small_* = max(2^-80, K w
+// at all (TreeArgs::wqkv_s null; loaded under a captured launch, every sum is
+// computed again), so a sum over K products of weights up to w is
+// off by at most K w 2^-134 from it: a sum below max(2^-80, K w
 // 2^-110), and one that is not finite, is computed again as float products.
 // Measured (d = 512, 8/2 heads of 64): QKV of 4096 rows 32 us (100 TFLOP/s of float
 // products), W_O 22; of 1024 rows 13 and 8.4.  Bound by what each wave does for
@@ -250,9 +250,11 @@ __global__ __launch_bounds__(256, NT > 2 ? 1 : 2) void proj_mma_kernel(TreeArgs 
         }
     // Thread: row tid / 8, columns 8 (tid % 8) .. + 7 of each 64 (all q, all k or all v).
     const int row = tid >> 3;
-    const float small = QKV ? a.small_qkv : a.small_wo;
+    const unsigned *range = a.range + (QKV ? 0 : 2);
+    const bool unfit = range[1] != 0;
+    const float small = fmaxf(0x1p-80f, (float)M * 0x1p-110f * __uint_as_float(range[0]));
     auto doubtful = [&](float y) {
-        return !(fabsf(y) >= small && fabsf(y) <= 3.4028235e38f) && y != 0.0f;
+        return unfit || (!(fabsf(y) >= small && fabsf(y) <= 3.4028235e38f) && y != 0.0f);
     };
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
@@ -1405,12 +1407,6 @@ template <bool QKV> void launch_proj_mma(const TreeArgs &a, int NC, hipStream_t 
 
 size_t split_weight_bytes(int K, int N) {
     return (size_t)((N + 31) / 32) * ((K + 15) / 16) * 3 * 1024;
-}
-
-float split_small_sum(int K, unsigned most) {
-    float w;
-    memcpy(&w, &most, sizeof w);
-    return std::max(0x1p-80f, (float)K * 0x1p-110f * w);
 }
 
 hipError_t launch_pack_split(const float *src, unsigned short *dst, int K, int N, int col0,

@@ -1354,3 +1354,43 @@ def test_tree_verify_one_order_of_sums(B):
         path, n_acc, nxt = [o.to_host() for o in out]
         assert (n_acc == int(accepted)).all(), n_acc
         assert (path == path[0]).all() and (nxt == nxt[0]).all()
+
+
+@pytest.mark.gpu
+def test_attn_tree_graph_after_new_weights():
+    """Weights loaded anew under a captured step: each replay computes with
+    the new ones' number range, which the split form of the projections may not
+    hold."""
+    print("[gpu-test] tree graph after new weights", flush=True)
+    B, N, d, nh, nkv, hd, S = 20, 8, 128, 8, 2, 16, 40
+    x, w, kc, vc, pos, c, s, par = tree_case(B, N, d, nh, nkv, hd, S, np.arange(B), 160, "tree")
+    x = (x * np.float32(1e14)).astype(np.float32)
+    at = mh.Attn(d, nh, nkv, hd, S)
+    load = lambda f: at.load(w["wq"], w["wk"], (w["wv"] * np.float32(f)).astype(np.float32), w["wo"], w["rms"])  # noqa: E731
+    load(1.0)
+    at.set_rope(c, s)
+    try:
+        run_tree(x, w, kc, vc, pos, c, s, par, nh, nkv, hd, at=at)
+        dx, dk, dv, dpar, dpos = dev(x), dev(kc), dev(vc), dev(par), dev(pos)
+        dy, gk, gv = mh.DeviceArray(x.shape), mh.DeviceArray((B, N, nkv * hd)), mh.DeviceArray((B, N, nkv * hd))
+        with mh.Graph() as g:
+            at.tree_dev(dx.ptr, dy.ptr, B, N, dpar.ptr, dpos.ptr, dk.ptr, dv.ptr, gk.ptr, gv.ptr, EPS)
+        try:
+            xn = x.astype(np.float64)
+            xn = xn / np.sqrt((xn ** 2).mean(2, keepdims=True) + EPS) * w["rms"]
+            for f in (1.0, 1e-36, 0.0, 1e20, 1.0):
+                load(f)
+                dy.zero(), gk.zero(), gv.zero()
+                g.launch()
+                mh.synchronize()
+                want = xn @ (w["wv"] * np.float32(f)).astype(np.float64)
+                if f:
+                    assert orc.rel_l2(gv.to_host() / f, want / f) <= 1e-6, f
+                else:
+                    assert not gv.to_host().any()
+                eager = run_tree(x, w, kc, vc, pos, c, s, par, nh, nkv, hd, at=at)
+                assert orc.rel_l2(eager[2] / (f or 1), gv.to_host() / (f or 1)) <= 1e-6
+        finally:
+            g.close()
+    finally:
+        at.close()
