@@ -336,7 +336,10 @@ int moe_hip_decode_block_dev(MoeHipAttn *attn, MoeHipLayer *layer, const float *
  * out: their rows of y, k_draft and v_draft stay as they were, and no other
  * row depends on theirs.  An infinity or NaN reaches only the nodes that
  * attend it.  Device pointers; x, y, caches and drafts 16-byte aligned.
- * Deterministic. */
+ * Deterministic.  The first call of more than 128 rows makes a form of the
+ * weights for many rows (6 bytes per weight, kept with attn) and waits for it;
+ * a call captured before any has made it projects its rows another way, as
+ * one of 128 does (other roundings, slower for hundreds of rows). */
 int moe_hip_attn_tree_dev(MoeHipAttn *attn, const float *x, float *y, int B, int N,
                           const int *parent, const int *pos, const float *k_cache,
                           const float *v_cache, float *k_draft, float *v_draft, float eps,

@@ -780,7 +780,8 @@ struct MoeHipAttn {
     // The projections' weights in 16-column tiles (when every width is a
     // multiple of 16): [wq | wk | wv] and wo, for the projection tiles.
     float *wqkv_p = nullptr, *wo_p = nullptr;
-    // And as three bf16 terms, for the projections of many rows (tree.hip).
+    // And as three bf16 terms, for the projections of many rows (tree.hip): made
+    // by the first call that takes them (split_weights), null before.
     unsigned short *wqkv_s = nullptr, *wo_s = nullptr;
     unsigned *range = nullptr;      // [4] their number ranges (launch_pack_split), and read back
     unsigned split_range[4] = {};
@@ -826,16 +827,44 @@ int moe_hip_attn_create(int d_model, int n_heads, int n_kv_heads, int head_dim, 
         moe_hip_attn_destroy(a);
         return set_err(MOE_HIP_ERR_NOMEM, "attention weights");
     }
-    const size_t qs = moe::split_weight_bytes(d_model, (int)(qd + 2 * kd));
-    const size_t os = moe::split_weight_bytes((int)qd, d_model);
-    if (hipMalloc(&a->wqkv_s, qs) != hipSuccess || hipMalloc(&a->wo_s, os) != hipSuccess ||
-        hipMalloc(&a->range, sizeof(a->split_range)) != hipSuccess ||
-        hipMemset(a->wqkv_s, 0, qs) != hipSuccess || hipMemset(a->wo_s, 0, os) != hipSuccess) {
-        moe_hip_attn_destroy(a);
-        return set_err(MOE_HIP_ERR_NOMEM, "attention weights");
-    }
     *out = a;
     return MOE_HIP_OK;
+}
+
+// Fills the split weights from the others, and waits.
+static int pack_split_weights(MoeHipAttn *a) {
+    const int d = a->d, q = a->nh * a->hd, kv = a->nkv * a->hd;
+    HIP_TRY(moe::launch_zero_ints(reinterpret_cast<int *>(a->range), 4, g_stream));
+    HIP_TRY(moe::launch_pack_split(a->wq, a->wqkv_s, d, q, 0, a->range, g_stream));
+    HIP_TRY(moe::launch_pack_split(a->wk, a->wqkv_s, d, kv, q, a->range, g_stream));
+    HIP_TRY(moe::launch_pack_split(a->wv, a->wqkv_s, d, kv, q + kv, a->range, g_stream));
+    HIP_TRY(moe::launch_pack_split(a->wo, a->wo_s, q, d, 0, a->range + 2, g_stream));
+    HIP_TRY(hipMemcpyAsync(a->split_range, a->range, sizeof(a->split_range), hipMemcpyDeviceToHost,
+                           g_stream));
+    HIP_TRY(hipStreamSynchronize(g_stream));
+    return MOE_HIP_OK;
+}
+
+// Makes the split weights (no stream may be capturing).
+static int split_weights(MoeHipAttn *a) {
+    if (a->wqkv_s) return MOE_HIP_OK;
+    const int q = a->nh * a->hd, kv = a->nkv * a->hd;
+    const size_t qs = moe::split_weight_bytes(a->d, q + 2 * kv), os = moe::split_weight_bytes(q, a->d);
+    int rc = MOE_HIP_OK;
+    if (hipMalloc(&a->wqkv_s, qs) != hipSuccess || hipMalloc(&a->wo_s, os) != hipSuccess ||
+        hipMalloc(&a->range, sizeof(a->split_range)) != hipSuccess)
+        rc = set_err(MOE_HIP_ERR_NOMEM, "attention weights for many rows");
+    else if (hipMemsetAsync(a->wqkv_s, 0, qs, g_stream) != hipSuccess ||
+             hipMemsetAsync(a->wo_s, 0, os, g_stream) != hipSuccess)
+        rc = set_err(MOE_HIP_ERR_HIP, "attention weights for many rows");
+    else
+        rc = pack_split_weights(a);
+    if (rc == MOE_HIP_OK) return rc;
+    for (void *p : {(void *)a->wqkv_s, (void *)a->wo_s, (void *)a->range})
+        if (p) (void)hipFree(p);
+    a->wqkv_s = a->wo_s = nullptr;
+    a->range = nullptr;
+    return rc;
 }
 
 int moe_hip_attn_load(MoeHipAttn *a, const float *wq, const float *wk, const float *wv,
@@ -853,16 +882,9 @@ int moe_hip_attn_load(MoeHipAttn *a, const float *wq, const float *wk, const flo
         HIP_TRY(moe::launch_pack_cols16(a->wk, a->wqkv_p, d, kv, q, g_stream));
         HIP_TRY(moe::launch_pack_cols16(a->wv, a->wqkv_p, d, kv, q + kv, g_stream));
         HIP_TRY(moe::launch_pack_cols16(a->wo, a->wo_p, q, d, 0, g_stream));
+        HIP_TRY(hipStreamSynchronize(g_stream));
     }
-    const int d = a->d, q = (int)qd, kv = (int)kd;
-    HIP_TRY(moe::launch_zero_ints(reinterpret_cast<int *>(a->range), 4, g_stream));
-    HIP_TRY(moe::launch_pack_split(a->wq, a->wqkv_s, d, q, 0, a->range, g_stream));
-    HIP_TRY(moe::launch_pack_split(a->wk, a->wqkv_s, d, kv, q, a->range, g_stream));
-    HIP_TRY(moe::launch_pack_split(a->wv, a->wqkv_s, d, kv, q + kv, a->range, g_stream));
-    HIP_TRY(moe::launch_pack_split(a->wo, a->wo_s, q, d, 0, a->range + 2, g_stream));
-    HIP_TRY(hipMemcpyAsync(a->split_range, a->range, sizeof(a->split_range), hipMemcpyDeviceToHost,
-                           g_stream));
-    HIP_TRY(hipStreamSynchronize(g_stream));
+    if (a->wqkv_s) TRY(pack_split_weights(a));
     return MOE_HIP_OK;
 }
 
@@ -1004,6 +1026,12 @@ int moe_hip_attn_tree_dev(MoeHipAttn *a, const float *x, float *y, int B, int N,
     TRY(g_ws.ao.reserve(sizeof(float) * (size_t)R * qd));
     TRY(g_ws.apart.reserve(sizeof(float) * plan.part_floats));
     TRY(g_ws.trow.reserve(sizeof(int) * (size_t)R));
+    // (a call captured before any that made them takes the other form)
+    if (R > moe::kTreeMmaRows && !g_api_capture) {
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        HIP_TRY(hipStreamIsCapturing(s, &cs));
+        if (cs == hipStreamCaptureStatusNone) TRY(split_weights(a));
+    }
     moe::TreeArgs t{};
     t.x = const_cast<float *>(x); t.y = y; t.rms_w = a->rms; t.eps = eps;
     t.wq = a->wq; t.wk = a->wk; t.wv = a->wv; t.wo = a->wo;

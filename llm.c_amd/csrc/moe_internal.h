@@ -265,6 +265,11 @@ hipError_t launch_pack_cols16(const float *src, float *dst, int K, int N, int co
 // [rows][kd] receive the nodes' keys and values, y [rows][d] (may be x) the
 // rows of x plus attention.
 constexpr int kTreeMaxNodes = 64;
+// Rows up to which the projections are proj16_kernel's, from there on
+// proj_mma_kernel's.  us per sublayer, both ways: d = 512, 8/2 heads of 64, 64 rows
+// 20.1 27.5, 128 22.1 26.1, 192 29.9 28.8, 512 48.7 32.2; d = 1024, 16/4 heads, 64
+// 28.7 35.3, 128 42.0 40.0, 256 74.0 49.5.
+constexpr int kTreeMmaRows = 128;
 struct TreeArgs : AttnArgs {
     int seqs = 0, N = 0;
     const int *parent = nullptr;   // [rows]

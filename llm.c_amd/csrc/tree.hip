@@ -61,11 +61,6 @@ constexpr float kLow = -3.0e38f;   // running maximum before the first score
 constexpr int kWaves = 4;
 constexpr int kMaxSplits = 128;
 constexpr long long kLittle = 1LL << 22;   // query rows times positions
-// Rows up to which the projections are proj16_kernel's, from there on
-// proj_mma_kernel's.  us per sublayer, both ways: d = 512, 8/2 heads of 64, 64 rows
-// 20.1 27.5, 128 22.1 26.1, 192 29.9 28.8, 512 48.7 32.2; d = 1024, 16/4 heads, 64
-// 28.7 35.3, 128 42.0 40.0, 256 74.0 49.5.
-constexpr int kMmaRows = 128;
 
 // ---------------------------------------------------------------------------
 // The tree of one sequence by a wave, lane base + i = node i.
@@ -1459,7 +1454,7 @@ hipError_t launch_attn_tree(const TreeArgs &a, hipStream_t s) {
     if (p.splits != a.splits || (p.part_floats && !a.part)) return hipErrorInvalidValue;
     const int NC = a.qd + 2 * a.kd;
     auto t16 = [](int n) { return (unsigned)((n + kPT - 1) / kPT); };
-    const bool small = a.B <= kPVRows, many = a.B > kMmaRows && a.wqkv_s && a.wo_s;
+    const bool small = a.B <= kPVRows, many = a.B > kTreeMmaRows && a.wqkv_s && a.wo_s;
     if (many)       launch_proj_mma<true>(a, NC, s);
     else if (small) hipLaunchKernelGGL((projv_kernel<true, TreeArgs>), dim3((unsigned)(NC / 4)), dim3(256), 0, s, a);
     else            hipLaunchKernelGGL((proj16_kernel<true, TreeArgs>), dim3(t16(NC), t16(a.B)), dim3(1024), 0, s, a);

@@ -1394,3 +1394,60 @@ def test_attn_tree_graph_after_new_weights():
             g.close()
     finally:
         at.close()
+
+
+@pytest.mark.gpu
+def test_attn_weights_for_many_rows_on_demand():
+    """The weights' form for projections of many rows is made by the first call
+    that takes it: a program that decodes holds two copies of its weights, not
+    three.  A call captured before that has its rows from the other form."""
+    print("[gpu-test] attention weights on demand", flush=True)
+    hip = C.CDLL(os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "lib", "libamdhip64.so"))
+
+    def free():
+        a, b = C.c_size_t(), C.c_size_t()
+        assert hip.hipMemGetInfo(C.byref(a), C.byref(b)) == 0
+        return a.value
+
+    mh.synchronize()
+    d, nh, nkv, hd = 4096, 64, 8, 64
+    weights = 4 * (2 * d * nh * hd + 2 * d * nkv * hd)
+    before = free()
+    at = mh.Attn(d, nh, nkv, hd, 16)
+    zero = [np.zeros(s, np.float32) for s in ((d, nh * hd), (d, nkv * hd), (d, nkv * hd), (nh * hd, d))]
+    at.load(*zero, np.ones(d, np.float32))
+    taken = before - free()
+    at.close()
+    # (two copies, of which small pieces may lie in memory that the runtime still
+    # held; three bf16 terms would be 1.5 times the weights more)
+    assert weights < taken < 2.3 * weights, (taken, weights)
+
+    B, N, d, nh, nkv, hd, S = 30, 6, 128, 8, 2, 16, 40
+    x, w, kc, vc, pos, c, s, par = tree_case(B, N, d, nh, nkv, hd, S, np.arange(B), 170, "holes")
+    ats = [mh.Attn(d, nh, nkv, hd, S) for _ in range(2)]
+    for at in ats:
+        at.load(w["wq"], w["wk"], w["wv"], w["wo"], w["rms"])
+        at.set_rope(c, s)
+    try:
+        first = run_tree(x, w, kc, vc, pos, c, s, par, nh, nkv, hd, at=ats[0], fill=0.0)   # (the workspace)
+        dx, dk, dv, dpar, dpos = dev(x), dev(kc), dev(vc), dev(par), dev(pos)
+        dy, gk, gv = mh.DeviceArray(x.shape), mh.DeviceArray((B, N, nkv * hd)), mh.DeviceArray((B, N, nkv * hd))
+        with mh.Graph() as g:
+            ats[1].tree_dev(dx.ptr, dy.ptr, B, N, dpar.ptr, dpos.ptr, dk.ptr, dv.ptr, gk.ptr, gv.ptr, EPS)
+        try:
+            seen = []
+            for it in range(3):
+                dy.zero(), gk.zero(), gv.zero()
+                g.launch()
+                mh.synchronize()
+                seen.append([t.to_host() for t in (dy, gk, gv)])
+                for u, v, e in zip(seen[0], seen[-1], first):
+                    assert np.array_equal(u, v) and orc.rel_l2(v, e) <= 1e-6
+                # (an eager call makes the other form, the graph keeps its own)
+                for u, v in zip(run_tree(x, w, kc, vc, pos, c, s, par, nh, nkv, hd, at=ats[1], fill=0.0), first):
+                    assert np.array_equal(u, v)
+        finally:
+            g.close()
+    finally:
+        for at in ats:
+            at.close()
