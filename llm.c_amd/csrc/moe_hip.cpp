@@ -769,6 +769,9 @@ int moe_hip_layer_load(MoeHipLayer *L, const MoEWeights *w) {
 
 static int forward_impl(MoeHipLayer *L, const float *x, int T, float *out, float *probs, int *ids,
                         int accumulate, void *stream, Norm nm);
+// What forward_impl refuses for T rows, and its workspace: for calls that queue
+// other work first.
+static int forward_ready(const MoeHipLayer *L, int T);
 
 // ---------------------------------------------------------------------------
 // Attention of the decode step (src/inference.c:252-308): weights in the
@@ -948,6 +951,7 @@ int moe_hip_decode_block_dev(MoeHipAttn *a, MoeHipLayer *L, const float *rms_ffn
         TRY(g_ws.xn.reserve(sizeof(float) * (size_t)B * L->d));
         xn = g_ws.xn.as<float>();
     }
+    TRY(forward_ready(L, B));
     TRY(attn_decode(a, x, B, pos, k_cache, v_cache, eps, stream));
     Norm nm;
     nm.x_raw = x; nm.rms_w = rms_ffn; nm.eps = eps;
@@ -1067,6 +1071,7 @@ int moe_hip_tree_block_dev(MoeHipAttn *a, MoeHipLayer *L, const float *rms_ffn, 
         TRY(g_ws.xn.reserve(sizeof(float) * (size_t)B * N * L->d));
         xn = g_ws.xn.as<float>();
     }
+    TRY(forward_ready(L, B * N));
     TRY(moe_hip_attn_tree_dev(a, x, x, B, N, parent, pos, k_cache, v_cache, k_draft, v_draft, eps,
                               stream));
     Norm nm;
@@ -1805,6 +1810,13 @@ static int forward_impl(MoeHipLayer *L, const float *x, int T, float *out, float
     FwdBufs b;
     TRY(workspace_bufs(L, p, &b));
     return run_forward(L, x, T, out, probs, ids, accumulate, s, nm, p, b);
+}
+
+static int forward_ready(const MoeHipLayer *L, int T) {
+    FwdPlan p;
+    TRY(plan_forward(L, T, &p, false));
+    FwdBufs b;
+    return workspace_bufs(L, p, &b);
 }
 
 // moe_hip_forward_dev on the fixed scratch array: no device memory is

@@ -1451,3 +1451,54 @@ def test_attn_weights_for_many_rows_on_demand():
     finally:
         for at in ats:
             at.close()
+
+
+@pytest.mark.gpu
+def test_block_refused_before_it_changes_rows():
+    """A block whose MoE half has more rows than it can index, or would grow
+    the workspace under a live graph, is refused with x and the drafts (or
+    the caches) as they were."""
+    print("[gpu-test] block refusals", flush=True)
+    d, F, nh, nkv, hd, S = 64, 8192, 4, 2, 16, 4
+    rng = np.random.default_rng(3)
+    at, layer = mh.Attn(d, nh, nkv, hd, S), mh.Layer(d, F, 2, 2)
+    at.load(*[rng.standard_normal(s).astype(np.float32) for s in ((d, 64), (d, 32), (d, 32), (64, d))], np.ones(d, np.float32))
+    at.set_rope(*orc.rope_tables(S, hd, 10000.0))
+    layer.fill_synthetic(1, 0.02, 0.02)
+    rms = dev(np.ones(d, np.float32))
+    L = mh.lib()
+    try:
+        B, N = 2048, 64                                     # 2^17 rows, 2^31 hidden values
+        x = rng.standard_normal((B * N, d)).astype(np.float32)
+        dx, par, pos = dev(x), dev(make_parents("chain", B, N, 0)), dev(np.zeros(B, np.int32))
+        cache = [mh.DeviceArray((B * N, S, nkv * hd)) for _ in range(2)]
+        draft = [mh.DeviceArray((B, N, nkv * hd)) for _ in range(2)]
+        for t in cache + draft:
+            t.zero()
+        kv, kvd = [t.ptr for t in cache], [t.ptr for t in draft]
+        rows = dev(np.zeros(B * N, np.int32))
+        assert L.moe_hip_tree_block_dev(at.h, layer.h, rms.ptr, dx.ptr, B, N, par.ptr, pos.ptr, *kv, *kvd, EPS, None, None, None) == 2
+        assert L.moe_hip_decode_block_dev(at.h, layer.h, rms.ptr, dx.ptr, B * N, rows.ptr, *kv, EPS, None, None, None) == 2
+        mh.synchronize()
+        assert np.array_equal(dx.to_host(), x)
+        assert not any(t.to_host().any() for t in draft + cache)
+        B = 1000
+        at.tree_dev(dx.ptr, mh.DeviceArray((B * N, d)).ptr, B, N, par.ptr, pos.ptr, *kv, *kvd, EPS)   # (its own workspace)
+        for t in draft:
+            t.zero()
+        big = mh.Layer(d, 16384, 2, 2)                      # (8 GB of hidden values)
+        big.fill_synthetic(1, 0.02, 0.02)
+        with mh.Graph() as g:
+            mh.fill_normal_dev(rms.ptr, 4, 1, 0, 1.0, 0.0)
+        try:
+            norm = mh.DeviceArray((B * N, d))
+            assert L.moe_hip_tree_block_dev(at.h, big.h, rms.ptr, dx.ptr, B, N, par.ptr, pos.ptr, *kv, *kvd, EPS,
+                                            norm.ptr, None, None) == 1
+            mh.synchronize()
+            assert np.array_equal(dx.to_host(), x) and not any(t.to_host().any() for t in draft)
+        finally:
+            g.close()
+            big.close()
+    finally:
+        at.close()
+        layer.close()
