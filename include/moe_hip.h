@@ -385,7 +385,7 @@ int moe_hip_tree_verify_dev(const float *p, size_t ldp, const float *q, size_t l
  * for j = 0 .. n_acc[b], cache row pos[b] + j of sequence b = draft row
  * path[b][j], for keys and values of every block (host arrays of n_blocks
  * device pointers: drafts [B][N][kv_dim], caches [B][max_seq][kv_dim], 16-byte
- * aligned, kv_dim a multiple of 4).  Rows that fall outside the cache and
+ * aligned, kv_dim a multiple of 4, drafts of at most 2^34 - 1024 floats).  Rows that fall outside the cache and
  * path entries outside [0, N) are left out, sequences with n_acc[b] < 0 or
  * pos[b] outside [0, max_seq) untouched.  pos_out [B] (NULL: not written)
  * receives pos[b] + n_acc[b] + 1, at most max_seq, or pos[b] for the

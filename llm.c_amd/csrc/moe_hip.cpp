@@ -1124,6 +1124,10 @@ int moe_hip_tree_commit_dev(int n_blocks, const float *const *k_draft, const flo
         return set_err(MOE_HIP_ERR_ARG, "n_blocks >= 0 and max_seq >= 1");
     if (kv_dim < 4 || kv_dim % 4)
         return set_err(MOE_HIP_ERR_UNSUPPORTED, "kv_dim must be a multiple of 4 (%d)", kv_dim);
+    // (a launch has fewer than 2^32 threads, one per four floats)
+    if ((unsigned long long)B * N * (kv_dim / 4) > (1ULL << 32) - 256)
+        return set_err(MOE_HIP_ERR_UNSUPPORTED, "B * N * kv_dim = %llu floats, at most 2^34 - 1024",
+                       (unsigned long long)B * N * kv_dim);
     if (B == 0) return MOE_HIP_OK;
     if (!pos || !path || !n_acc || (n_blocks > 0 && (!k_draft || !v_draft || !k_cache || !v_cache)))
         return set_err(MOE_HIP_ERR_ARG, "null argument");

@@ -1502,3 +1502,12 @@ def test_block_refused_before_it_changes_rows():
     finally:
         at.close()
         layer.close()
+
+
+def test_commit_refuses_launches_past_the_grid_without_gpu():
+    """Drafts of more float4s than a launch has threads are refused, before
+    anything touches a device."""
+    L, P = mh.lib(), C.c_void_p
+    arrs = [(P * 1)(v << 44) for v in range(1, 5)]
+    for B, N, kd in ((8192, 64, 32768), (1 << 19, 1, 32768), (1, 64, 2147483644)):
+        assert L.moe_hip_tree_commit_dev(1, *arrs, B, N, kd, 8, P(4096), P(1 << 30), P(1 << 31), None, None) == 2
