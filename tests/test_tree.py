@@ -1511,3 +1511,29 @@ def test_commit_refuses_launches_past_the_grid_without_gpu():
     arrs = [(P * 1)(v << 44) for v in range(1, 5)]
     for B, N, kd in ((8192, 64, 32768), (1 << 19, 1, 32768), (1, 64, 2147483644)):
         assert L.moe_hip_tree_commit_dev(1, *arrs, B, N, kd, 8, P(4096), P(1 << 30), P(1 << 31), None, None) == 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("block", range(10))
+def test_random_drafted_shapes(block):
+    """Seeded random shapes of attention (head shapes, widths, trees, positions
+    inside and outside the cache, small and large calls) and of verification
+    (vocabularies up to 90000), ten of each."""
+    for seed in range(5000 + 10 * block, 5010 + 10 * block):
+        rng = np.random.default_rng(seed)
+        nkv, G, hd = int(rng.integers(1, 5)), int(rng.integers(1, 9)), 8 * int(rng.integers(1, 9))
+        N = int(rng.integers(1, 65)) if rng.random() < 0.6 else int(rng.integers(1, 9))
+        B = int(np.exp(rng.uniform(0, np.log(max(2, min(200, 1500 // N))))))
+        d = 4 * int(rng.integers(2, 100))
+        S = int(np.exp(rng.uniform(np.log(2), np.log(700 if B * N < 400 else 150))))
+        kind = rng.choice(["chain", "tree", "forest", "holes", "ragged", "star", "none"])
+        pos = rng.integers(-1 if rng.random() < 0.3 else 0, S + (1 if rng.random() < 0.3 else 0), B)
+        many = "many" if rng.random() < 0.6 and N * nkv * hd * 4 * (2 ** 22 // max(1, B * N * nkv * G)) * B < 3e8 else "few"
+        print(f"[gpu-test] seed {seed}: tree {(B, N, d, nkv * G, nkv, hd, S)} {kind} {many}", flush=True)
+        check_tree(*tree_case(B, N, d, nkv * G, nkv, hd, S, pos, seed, kind, many), nkv * G, nkv, hd, in_place=bool(rng.random() < 0.3))
+        V = int(np.exp(rng.uniform(0, np.log(90000))))
+        B = int(rng.integers(1, max(2, min(80, 3000000 // (V * min(N, 20))))))
+        N = min(N, 20) if V > 2000 else N
+        probs, kind = bool(rng.random() < 0.7), rng.choice(["chain", "tree", "forest", "holes", "ragged", "star"])
+        print(f"[gpu-test] seed {seed}: verify {(B, N, V)} {kind} {probs}", flush=True)
+        check_verify(*verify_case(B, N, V, kind, seed, probs, float(rng.uniform(0.2, 4))), pad=int(rng.integers(0, 4)))
