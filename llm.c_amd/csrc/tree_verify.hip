@@ -39,9 +39,9 @@
 //     (no differences of nearly equal sums).
 //   - the walk itself is a few instructions per child tried: every wave holds
 //     the nodes, one per lane.
-// Measured: 64 trees of 32 nodes over 131072 tokens 46 us (the last sequence's
+// Measured: 64 trees of 32 nodes over 131072 tokens 48-50 us (the last sequence's
 // five passes, 5 us of reading and 3 us of handing over each; 79 us with the first
-// pass shared only), 64 of 16 over 32768 21 us, one chain of 6 over 4096 7.5 us
+// pass shared only), 64 of 16 over 32768 23-26 us, one chain of 6 over 4096 7.5 us
 // (the launch), 33 trees of 24 looked-up nodes over 50001 13 us.
 #include "handoff.h"
 #include "moe_internal.h"
@@ -287,47 +287,31 @@ template <int WAVES> __device__ void sum_list(double a, int s0, int s1, VerifySm
 // The same, each lane taking what was its own, in order: the bits that sum_segs
 // gives (the tokens left out add 0).  Lanes keep only what still counts: the
 // first pass takes the longest lane's number of steps, up to 16, the later ones
-// some 7.  A wave's segments four at a time.
+// some 7 (64 trees of 16 over 131072 tokens 49.9 us; pairs to the lanes in turn
+// 45.8, but then the bits hang on who adds up the part).
 template <int WAVES> __device__ void sum_lanes(double a, int s0, int s1, VerifySmem &sm) {
-    constexpr int G = 4;
+    constexpr int U = 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    unsigned short *words = sm.lanes(s1 - s0) + lane;
-    for (int s = s0 + wave; s < s1; s += G * WAVES) {
-        int own[G], at[G], n[G], most = 0;
-        double t[G];
+    for (int s = s0 + wave; s < s1; s += WAVES) {
+        unsigned short *word = sm.lanes(s1 - s0) + (s - s0) * 64 + lane;
+        const int w = *word, own = w & 31, at = sm.off[s] + (w >> 5);
+        int n = 0;
+        double t = 0.0;
+        for (int i = 0; __any(i < own); i += U) {
+            float2 v[U];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int x = min(s + g * WAVES, s1 - 1), w = words[(x - s0) * 64];
-            own[g] = s + g * WAVES < s1 ? w & 31 : 0;
-            at[g] = sm.off[x] + (w >> 5);
-            n[g] = 0;
-            t[g] = 0.0;
-            most = max(most, own[g]);
+            for (int u = 0; u < U; ++u) v[u] = sm.list[i + u < own ? at + i + u : kListZero];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const double r = left_of(v[u].x, v[u].y, a);
+                t += r;
+                sm.list[i + u < own ? at + n : kListZero + 1] = v[u];
+                n += r > 0.0;
+            }
         }
-        for (int i = 0; __any(i < most); i += 2) {
-            float2 v[G][2];
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) v[g][u] = sm.list[i + u < own[g] ? at[g] + i + u : kListZero];
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const double r = left_of(v[g][u].x, v[g][u].y, a);
-                    t[g] += r;
-                    sm.list[i + u < own[g] ? at[g] + n[g] : kListZero + 1] = v[g][u];
-                    n[g] += r > 0.0;
-                }
-        }
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            if (s + g * WAVES >= s1) break;
-            unsigned short *w = words + (s + g * WAVES - s0) * 64;
-            *w = (unsigned short)((*w & ~31) | n[g]);
-            const double all = wave_sum64(t[g]);
-            if (lane == 0) sm.seg[s + g * WAVES] = all;
-        }
+        *word = (unsigned short)((w & ~31) | n);
+        t = wave_sum64(t);
+        if (lane == 0) sm.seg[s] = t;
     }
 }
 
@@ -783,11 +767,12 @@ VerifyPlan verify_plan(int B, int V, bool has_q) {
     // A workgroup per CU, of eight segments at least.
     p.parts = std::min({std::max(1, device_cus() / std::max(B, 1)), (p.segs + 7) / 8, kVerifyParts});
     // Later passes with help: a hand-over costs 3 us, a CU alone reads a segment
-    // of both rows in 0.18.  us (trees of 16, alone and together) with 8
-    // sequences over 16384 tokens 14.2 19.2, 65536 25.6 20.2, 262144 63.3 21.1; 64
-    // sequences (4 parts) 32768 21.1 28.1, 65536 29.6 25.4, 131072 67.1 45.3; 100
-    // (2 parts) 65536 34.4 37.5.  Without q nodes rarely need more than one pass:
-    // 8 over 262144 14.1 15.7.
+    // of both rows in 0.18.  us (trees of 16, alone and together, mean of six
+    // seeds) with one sequence over 65536 tokens 15.3 16.5, 131072 18.0 13.0; 8
+    // sequences 65536 22.4 22.0, 131072 36.5 23.8; 64 sequences (4 parts) 65536
+    // 32.8 33.3, 131072 65.0 49.9.  Below that it loses (64 over 32768 22 35), and
+    // with two parts too (100 over 65536 34 38).  Without q nodes rarely need more
+    // than one pass: 8 over 262144 14.1 15.7.
     p.together = has_q && p.parts >= 4 && p.segs >= 64;
     p.sum_bytes = p.parts > 1 ? (size_t)B * (p.segs + kTreeMaxNodes) * 8 : 0;
     p.word_bytes = p.parts > 1 ? (size_t)B * sizeof(VerifyWords) : 0;
