@@ -336,10 +336,18 @@ int moe_hip_decode_block_dev(MoeHipAttn *attn, MoeHipLayer *layer, const float *
  * out: their rows of y, k_draft and v_draft stay as they were, and no other
  * row depends on theirs.  An infinity or NaN reaches only the nodes that
  * attend it.  Device pointers; x, y, caches and drafts 16-byte aligned.
- * Deterministic.  The first call of more than 128 rows makes a form of the
- * weights for many rows (6 bytes per weight, kept with attn) and waits for it;
- * a call captured before any has made it projects its rows another way, as
- * one of 128 does (other roundings, slower for hundreds of rows). */
+ * Deterministic.
+ * Rounding: with more than 32 query rows (N times query heads per kv head) in
+ * all but small calls, the attention's products take each operand as two fp16
+ * terms, 22 bits: a score is off by about 2^-22 of its products' magnitudes,
+ * about what a chain of float products gives.  Where the terms do not hold
+ * enough (numbers out of their range, small ones beside large ones where that
+ * would show) a range of positions is computed as float products, some five
+ * times slower.
+ * The first call of more than 128 rows makes a form of the weights for many
+ * rows (6 bytes per weight, kept with attn) and waits for it; a call captured
+ * before any has made it projects its rows as one of 128 does (other roundings,
+ * slower for hundreds of rows). */
 int moe_hip_attn_tree_dev(MoeHipAttn *attn, const float *x, float *y, int B, int N,
                           const int *parent, const int *pos, const float *k_cache,
                           const float *v_cache, float *k_draft, float *v_draft, float eps,
@@ -376,7 +384,9 @@ int moe_hip_tree_block_dev(MoeHipAttn *attn, MoeHipLayer *layer, const float *rm
  * are passed over.  Entries that are negative or NaN count as 0 once the
  * recursion subtracts or sums them.  next[b] = -1 where the sum to draw from
  * is zero or not finite.  A sequence whose parent[b][0] is not -1 gets
- * n_acc[b] = next[b] = -1 and a path of -1. */
+ * n_acc[b] = next[b] = -1 and a path of -1.  Every node counts whose parents
+ * lead to node 0: mark those whose position is past the cache (their rows are
+ * not the target's) as no token.  Deterministic. */
 int moe_hip_tree_verify_dev(const float *p, size_t ldp, const float *q, size_t ldq, int B, int N,
                             int V, const int *parent, const int *token, const float *u_accept,
                             const float *u_sample, int *path, int *n_acc, int *next, void *stream);

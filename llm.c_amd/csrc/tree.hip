@@ -622,7 +622,7 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeArgs a, int block
 // of it at worst, where the float products' chain rounds its running sum at
 // 2^-24 eight times as often.  (Three bf16 terms hold all 24 bits at any scale but cost
 // six products and 11 instead of 4 VALU instructions per pair split: 120 us
-// where this form takes 80 us for trees of 64 over 2048 positions, 64 sequences.)  fp16's
+// where this form takes 83 us for trees of 64 over 2048 positions, 64 sequences.)  fp16's
 // range is narrow, so operands are scaled by powers of two first, which is exact:
 //   Q   each row to a maximum in [2^11, 2^12);
 //   K   the range's first tile to [2^8, 2^9), the later ones by the same factor; its
@@ -655,10 +655,12 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeArgs a, int block
 //   O^T = V^T P^T  the accumulators of S^T are the B operand: element j of k
 //                  step t, lane half h, is register 8 t + j, position 8 (2 t +
 //                  j / 4) + 4 h + j % 4, and V is laid out to match.
-// Measured (8/2 heads of 64): 64 trees of 64 over 2048 positions 80 us, 188
-// TFLOP/s of float products (the matrix cores 33 % busy; exponentials and
-// splitting beside them); 64 of 16 over 1024 26 us; two of 32 over 32768 30 us,
-// 64 MB at 2.2 TB/s.
+// Measured (8/2 heads of 64): 64 trees of 64 over 2048 positions 83 us, 182
+// TFLOP/s of float products (the matrix cores 32 % busy; exponentials and
+// splitting beside them); 64 of 16 over 1024 27 us; two of 32 over 32768 32 us,
+// 64 MB at 2.1 TB/s.  The rules for taking a range again cost 2 % of a call (64
+// shuffles at its end); where every range is taken again the three calls of those
+// shapes take 847 instead of 155, 157 instead of 55 and 233 instead of 50 us.
 typedef _Float16 hx2 __attribute__((ext_vector_type(2)));
 typedef _Float16 hx8 __attribute__((ext_vector_type(8)));
 typedef float fx2 __attribute__((ext_vector_type(2)));
@@ -1420,10 +1422,12 @@ TreePlan tree_plan(int seqs, int N, int nh, int nkv, int hd, int max_seq) {
     // (from 33 on split, tree_attn_split_kernel), unless the whole call is
     // little: then it is the length of one wave's work that counts.  us per
     // sublayer with 16, 32, 64, 128 (heads of 64, 4 per kv head): one sequence
-    // of 1024 positions, N = 8 20.1 22.3 22.8 22.6, N = 32 21.1 22.8 23.3 23.6; four
-    // of 4096, N = 16 28.4 28.6 32.0 31.2, N = 32 36.8 38.6 37.4 37.8, N = 64 50.9
-    // 50.7 46.5 43.4; 64 of 1024, N = 8 43.1 42.7 46.2 46.4, N = 16 64.0 51.4 50.1
-    // 51.3, N = 32 114 89.1 72.4 67.5; 256 of 1024, N = 8 116 89.9 90.8 101.
+    // of 1024 positions, N = 8 20.1 22.5 23.9 23.7, N = 32 21.0 22.9 24.3 24.6; four
+    // of 4096, N = 16 28.2 28.4 33.1 32.2, N = 32 36.5 38.3 38.6 39.0, N = 64 49.3
+    // 49.6 46.2 43.1; 64 of 1024, N = 8 43.9 41.2 46.4 46.5, N = 16 66.3 50.7 51.1
+    // 51.4, N = 32 115 85.4 70.1 65.8; 256 of 1024, N = 8 119 88.5 96.3 104.
+    // Positions are counted as the cache's capacity: where the sequences are in it
+    // is known to the device only.
     const bool little = (long long)seqs * nkv * rows * max_seq < kLittle;
     p.rows = rows <= 16 || little ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128;
     p.blocks = (rows + p.rows - 1) / p.rows;
@@ -1432,11 +1436,13 @@ TreePlan tree_plan(int seqs, int N, int nh, int nkv, int hd, int max_seq) {
     // One workgroup per CU where a wave takes whole rows alone, two where four
     // share their tiles (their barriers leave gaps), a tile per wave at least.
     // us per sublayer by workgroups per CU, 1/2, 1, 2, 4 (d = 512, 8/2 heads of
-    // 64): 64 sequences of 1024 positions, N = 1 28.1 27.9 30.3 34.7, N = 16 60.0
-    // 50.8 50.1 61.4, N = 32 83.7 69.7 67.4 79.3; of 2048, N = 64 143 143 130 138;
-    // one of 1024, N = 32 23.8 21.2 21.7 21.6.  By the splits allowed, 32, 64,
-    // 128: one sequence of 32768, N = 32 62.1 44.1 37.5; of 65536, N = 16 78.2
-    // 52.8 42.7.
+    // 64): 64 sequences of 1024 positions, N = 1 27.8 29.2 30.3 34.4, N = 16 61.2
+    // 51.5 51.0 64.0, N = 32 82.6 68.4 66.0 78.3; of 2048, N = 64 144 145 129 137;
+    // one of 1024, N = 32 23.4 21.0 21.7 21.7.  By the splits allowed, 32, 64,
+    // 128: one sequence of 32768, N = 32 65.2 45.8 38.1; of 65536, N = 16 83.0
+    // 55.8 43.8.  A sequence at position 1000 takes 20.2 us in a cache of 1100,
+    // 25.0 in one of 131072 (N = 8; N = 32 20.9 and 29.1): most of its 128 splits
+    // are empty.
     const long long goal = (p.rows <= 32 ? 1LL : 2LL) * device_cus();
     const long long want = (goal + base - 1) / base, most = (tiles + kWaves - 1) / kWaves;
     p.splits = (int)std::max(1LL, std::min(std::min(want, most), (long long)kMaxSplits));
