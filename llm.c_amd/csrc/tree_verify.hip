@@ -94,7 +94,8 @@ __device__ inline double wave_back_scan64(double v, int lane) {   // of the lane
     return v;
 }
 // What is left of the target's distribution at one node: r(x) from p(x) and
-// q(x); with q null p(x), less the tokens that gone holds.
+// q(x); with q null p(x), less the tokens that gone holds.  No less than 0, and
+// what is no number is 0; q likewise, so that r only falls as a grows.
 struct Left {
     const float *p, *q;
     double a;
@@ -102,7 +103,7 @@ struct Left {
     int ngone;
 };
 __device__ inline double left_of(float p, float q, double a) {
-    return fmax(fma(-a, (double)q, (double)p), 0.0);   // (NaN: 0)
+    return fmax(fma(-a, (double)fmaxf(q, 0.0f), (double)p), 0.0);
 }
 
 struct VerifySmem {
@@ -439,7 +440,7 @@ __global__ __launch_bounds__(THREADS) void tree_verify_kernel(VerifyArgs a, Veri
         sm.token[tid] = t;
         sm.u[tid] = a.u_accept[row0 + tid];
         sm.pt[tid] = child ? a.p[(row0 + par) * a.ldp + t] : 0.0f;
-        sm.qt[tid] = child ? (has_q ? a.q[(row0 + par) * a.ldq + t] : 1.0f) : 0.0f;
+        sm.qt[tid] = child ? (has_q ? fmaxf(a.q[(row0 + par) * a.ldq + t], 0.0f) : 1.0f) : 0.0f;
         sm.path[tid] = -1;
     }
     __syncthreads();

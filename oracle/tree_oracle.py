@@ -82,7 +82,7 @@ def verify(p, q, parent, token, u_accept, u_sample):
                     t = int(token[b, c])
                     if parent[b, c] != cur or not 0 <= t < V:
                         continue
-                    drawn = np.zeros(V) if q is None else q[b, cur].astype(np.float64)
+                    drawn = np.zeros(V) if q is None else pos0(q[b, cur].astype(np.float64))
                     if q is None:
                         drawn[t] = 1.0
                     if float(u_accept[b, c]) * drawn[t] < pos0(left[t] / total):

@@ -1537,3 +1537,24 @@ def test_random_drafted_shapes(block):
         probs, kind = bool(rng.random() < 0.7), rng.choice(["chain", "tree", "forest", "holes", "ragged", "star"])
         print(f"[gpu-test] seed {seed}: verify {(B, N, V)} {kind} {probs}", flush=True)
         check_verify(*verify_case(B, N, V, kind, seed, probs, float(rng.uniform(0.2, 4))), pad=int(rng.integers(0, 4)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(12, 10, 300), (3, 14, 9000), (4, 8, 70001), (64, 4, 66000)], ids=lambda s: "_".join(map(str, s)))
+def test_tree_verify_no_numbers_in_q(shape):
+    """Entries of q that are negative or NaN count as 0, like p's: nothing is
+    taken off a token there, in the first pass over a row and in those from
+    lists."""
+    B, N, V = shape
+    print(f"[gpu-test] verify no numbers in q {shape}", flush=True)
+    p, q, par, tok, ua, us = verify_case(B, N, V, "star", 23)
+    ua = np.maximum(ua, 0.9).astype(np.float32)
+    q[:, :, 3::40] = -0.25
+    q[:, :, 5::40] = np.nan
+    q[:, :, 7::90] = -np.inf
+    p[:, :, 11::80] = -0.5                       # (both negative)
+    q[:, :, 11::80] = -0.4
+    p[:, :, 13::80] = np.nan
+    q[:, :, 13::80] = -0.3
+    for t in (tok, np.where(np.arange(N) % 3 == 2, tok // 40 * 40 + 3, tok), np.where(np.arange(N) % 3 == 1, tok // 40 * 40 + 5, tok)):
+        check_verify(p, q, par, np.minimum(t, V - 1).astype(np.int32), ua, us)
