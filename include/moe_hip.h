@@ -340,7 +340,8 @@ int moe_hip_decode_block_dev(MoeHipAttn *attn, MoeHipLayer *layer, const float *
  * Rounding: with more than 32 query rows (N times query heads per kv head) in
  * all but small calls, the attention's products take each operand as two fp16
  * terms, 22 bits: a score is off by about 2^-22 of its products' magnitudes,
- * about what a chain of float products gives.  Where the terms do not hold
+ * about what a chain of float products gives.  Values from 2^90 on may sum to
+ * infinity with 32 query rows or fewer, before they are divided.  Where the terms do not hold
  * enough (numbers out of their range, small ones beside large ones where that
  * would show) a range of positions is computed as float products, some five
  * times slower.
@@ -395,9 +396,9 @@ int moe_hip_tree_verify_dev(const float *p, size_t ldp, const float *q, size_t l
  * for j = 0 .. n_acc[b], cache row pos[b] + j of sequence b = draft row
  * path[b][j], for keys and values of every block (host arrays of n_blocks
  * device pointers: drafts [B][N][kv_dim], caches [B][max_seq][kv_dim], 16-byte
- * aligned, kv_dim a multiple of 4, drafts of at most 2^34 - 1024 floats).  Rows that fall outside the cache and
- * path entries outside [0, N) are left out, sequences with n_acc[b] < 0 or
- * pos[b] outside [0, max_seq) untouched.  pos_out [B] (NULL: not written)
+ * aligned, kv_dim a multiple of 4, drafts of at most 2^34 - 1024 floats).
+ * Rows that fall outside the cache and path entries outside [0, N) are left out,
+ * sequences with n_acc[b] < 0 or pos[b] outside [0, max_seq) untouched.  pos_out [B] (NULL: not written)
  * receives pos[b] + n_acc[b] + 1, at most max_seq, or pos[b] for the
  * untouched; it may be pos itself. */
 int moe_hip_tree_commit_dev(int n_blocks, const float *const *k_draft, const float *const *v_draft,

@@ -1133,6 +1133,7 @@ int moe_hip_tree_commit_dev(int n_blocks, const float *const *k_draft, const flo
         return set_err(MOE_HIP_ERR_ARG, "null argument");
     const size_t db = sizeof(float) * (size_t)B * N * kv_dim;
     const size_t cb = sizeof(float) * (size_t)B * max_seq * kv_dim;
+    const size_t pb = sizeof(int) * (size_t)B, nb = pb * N;
     for (int l = 0; l < n_blocks; ++l) {
         for (const float *p : {k_draft[l], v_draft[l], (const float *)k_cache[l],
                                (const float *)v_cache[l]})
@@ -1150,8 +1151,11 @@ int moe_hip_tree_commit_dev(int n_blocks, const float *const *k_draft, const flo
             }
         if (overlap(k_cache[l], cb, v_cache[l], cb))
             return set_err(MOE_HIP_ERR_ARG, "block %d: its caches overlap", l);
+        if (clash({{k_cache[l], cb}, {v_cache[l], cb}}, {{pos, pb}, {path, nb}, {n_acc, pb}}))
+            return set_err(MOE_HIP_ERR_ARG, "block %d: its caches overlap pos, path or n_acc", l);
+        if (pos_out && clash({{pos_out, pb}}, {{k_draft[l], db}, {v_draft[l], db}, {k_cache[l], cb}, {v_cache[l], cb}}))
+            return set_err(MOE_HIP_ERR_ARG, "pos_out and the rows of block %d overlap", l);
     }
-    const size_t pb = sizeof(int) * (size_t)B, nb = pb * N;
     if (pos_out && ((pos_out != pos && overlap(pos_out, pb, pos, pb)) ||
                     overlap(pos_out, pb, path, nb) || overlap(pos_out, pb, n_acc, pb)))
         return set_err(MOE_HIP_ERR_ARG, "pos_out must be pos or apart from the other arrays");

@@ -1558,3 +1558,20 @@ def test_tree_verify_no_numbers_in_q(shape):
     q[:, :, 13::80] = -0.3
     for t in (tok, np.where(np.arange(N) % 3 == 2, tok // 40 * 40 + 3, tok), np.where(np.arange(N) % 3 == 1, tok // 40 * 40 + 5, tok)):
         check_verify(p, q, par, np.minimum(t, V - 1).astype(np.int32), ua, us)
+
+
+def test_commit_refuses_overlaps_with_whole_numbers_without_gpu():
+    """Caches over positions, paths or counts, and positions written over
+    drafts or caches, are refused."""
+    L, P = mh.lib(), C.c_void_p
+    B, N, kd, S = 4, 8, 16, 10                      # drafts of 2 KB, caches of 2.5 KB
+
+    def commit(kc=0x30000, vc=0x40000, kdr=0x50000, vdr=0x60000, pos=0x10000, path=0x11000, n_acc=0x12000, out=0x13000):
+        arrs = [(P * 2)(a, a + 0x100000) for a in (kdr, vdr, kc, vc)]
+        return L.moe_hip_tree_commit_dev(2, *arrs, B, N, kd, S, P(pos), P(path), P(n_acc), P(out), None)
+
+    for what in ("pos", "path", "n_acc"):
+        for at in (0x30000, 0x30000 + 2556, 0x40010, 0x130020, 0x140020):
+            assert commit(**{what: at}) == 1, (what, hex(at))
+    for at in (0x30000, 0x40010, 0x50000 + 2044, 0x60000, 0x130020, 0x150020):
+        assert commit(out=at) == 1, hex(at)
