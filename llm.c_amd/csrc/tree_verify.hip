@@ -39,7 +39,7 @@
 //     (no differences of nearly equal sums).
 //   - the walk itself is a few instructions per child tried: every wave holds
 //     the nodes, one per lane.
-// Measured: 64 trees of 32 nodes over 131072 tokens 48-50 us (the last sequence's
+// Measured: 64 trees of 32 nodes over 131072 tokens 47-54 us (the last sequence's
 // five passes, 5 us of reading and 3 us of handing over each; 79 us with the first
 // pass shared only), 64 of 16 over 32768 23-26 us, one chain of 6 over 4096 7.5 us
 // (the launch), 33 trees of 24 looked-up nodes over 50001 13 us.
@@ -288,8 +288,8 @@ template <int WAVES> __device__ void sum_list(double a, int s0, int s1, VerifySm
 // The same, each lane taking what was its own, in order: the bits that sum_segs
 // gives (the tokens left out add 0).  Lanes keep only what still counts: the
 // first pass takes the longest lane's number of steps, up to 16, the later ones
-// some 7 (64 trees of 16 over 131072 tokens 49.9 us; pairs to the lanes in turn
-// 45.8, but then the bits hang on who adds up the part).
+// some 7 (64 trees of 16 over 131072 tokens 49.9 us where pairs to the lanes in
+// turn took 45.8, but then the bits hang on who adds up the part).
 template <int WAVES> __device__ void sum_lanes(double a, int s0, int s1, VerifySmem &sm) {
     constexpr int U = 2;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -769,11 +769,11 @@ VerifyPlan verify_plan(int B, int V, bool has_q) {
     p.parts = std::min({std::max(1, device_cus() / std::max(B, 1)), (p.segs + 7) / 8, kVerifyParts});
     // Later passes with help: a hand-over costs 3 us, a CU alone reads a segment
     // of both rows in 0.18.  us (trees of 16, alone and together, mean of six
-    // seeds) with one sequence over 65536 tokens 15.3 16.5, 131072 18.0 13.0; 8
-    // sequences 65536 22.4 22.0, 131072 36.5 23.8; 64 sequences (4 parts) 65536
-    // 32.8 33.3, 131072 65.0 49.9.  Below that it loses (64 over 32768 22 35), and
-    // with two parts too (100 over 65536 34 38).  Without q nodes rarely need more
-    // than one pass: 8 over 262144 14.1 15.7.
+    // seeds) with one sequence over 65536 tokens 16.2 17.3, 131072 19.4 15.2; 8
+    // sequences 65536 23.6 22.3, 131072 38.9 25.1; 64 sequences (4 parts) 65536
+    // 34.5 34.4, 131072 69.5 51.0.  Below that it loses (8 over 16384 16.0 23.8, 64
+    // over 32768 24.2 31.4), and with two parts too (100 over 65536 41.5 48.9).
+    // Without q nodes rarely need more than one pass: 8 over 262144 14.1 15.7.
     p.together = has_q && p.parts >= 4 && p.segs >= 64;
     p.sum_bytes = p.parts > 1 ? (size_t)B * (p.segs + kTreeMaxNodes) * 8 : 0;
     p.word_bytes = p.parts > 1 ? (size_t)B * sizeof(VerifyWords) : 0;
