@@ -340,8 +340,7 @@ int moe_hip_decode_block_dev(MoeHipAttn *attn, MoeHipLayer *layer, const float *
  * Rounding: with more than 32 query rows (N times query heads per kv head) in
  * all but small calls, the attention's products take each operand as two fp16
  * terms, 22 bits: a score is off by about 2^-22 of its products' magnitudes,
- * about what a chain of float products gives.  Values from 2^90 on may sum to
- * infinity with 32 query rows or fewer, before they are divided.  Where the terms do not hold
+ * about what a chain of float products gives.  Where the terms do not hold
  * enough (numbers out of their range, small ones beside large ones where that
  * would show) a range of positions is computed as float products, some five
  * times slower.

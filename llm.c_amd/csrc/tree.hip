@@ -568,22 +568,48 @@ __global__ __launch_bounds__(256, 2) void tree_attn_kernel(TreeArgs a, int block
         if (t + 2 < t1) step(S2{}, t + 2);
     }
 
-    // The waves' partial outputs, in wave order.
+    // The wave's partial outputs; true where one is not finite.
+    auto put = [&](bool again) {
+        bool more = false;
 #pragma unroll
-    for (int c = 0; c < QT; ++c) {
-        float x = l[c] + __shfl_xor(l[c], 16);
-        x += __shfl_xor(x, 32);
-        if (g == 0) {
-            sm_m[wave][16 * c + li] = m[c];
-            sm_l[wave][16 * c + li] = x;
+        for (int c = 0; c < QT; ++c) {
+            float x = l[c] + __shfl_xor(l[c], 16);
+            x += __shfl_xor(x, 32);
+            if (g == 0 && !again) {
+                sm_m[wave][16 * c + li] = m[c];
+                sm_l[wave][16 * c + li] = x;
+            }
+            const float inv = part_inv(x);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    float &out = sm_o[wave][16 * c + li][DT * (4 * g + r) + d];
+                    if (!again || !(fabsf(out) < INFINITY)) out = o[c][d][r] * inv;
+                    more |= !(fabsf(o[c][d][r]) < INFINITY) && m[c] < INFINITY;
+                }
         }
-        const float inv = part_inv(x);
+        return more;
+    };
+    // Values from 2^92 or so on may sum to infinity, as a probability is up to
+    // 2^kSlack: then the range once more, tile by tile, with maxima so high that
+    // the probabilities' sum is 1 at most, for the dimensions that need it.
+    if (__any(put(false))) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+        for (int c = 0; c < QT; ++c) {
+            m[c] += kSlack + 20.0f;   // (fewer than 2^20 positions)
+            l[c] = 0.0f;
 #pragma unroll
-            for (int d = 0; d < DT; ++d)
-                sm_o[wave][16 * c + li][DT * (4 * g + r) + d] = o[c][d][r] * inv;
+            for (int d = 0; d < DT; ++d) o[c][d] = fx4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+#pragma unroll 1
+        for (int t = t0; t < t1; ++t) {
+            load(S0{}, t);
+            step(S0{}, t);
+        }
+        put(true);
     }
+    // The waves' outputs, in wave order.
     __syncthreads();
     const size_t bk = (size_t)b * a.nkv + kvh;
     for (int e = tid; e < ROWS * HD; e += 256) {

@@ -1575,3 +1575,24 @@ def test_commit_refuses_overlaps_with_whole_numbers_without_gpu():
             assert commit(**{what: at}) == 1, (what, hex(at))
     for at in (0x30000, 0x40010, 0x50000 + 2044, 0x60000, 0x130020, 0x150020):
         assert commit(out=at) == 1, hex(at)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [1, 3, 4, 8, 12, 40])
+def test_attn_tree_values_near_the_largest(N, positions):
+    """Cached values of 1e37 and scores that grow along the context: sums before
+    the division stay finite in every block size, outputs are the definition's
+    (W_O = 1e-37)."""
+    B, nh, nkv, hd, S = 3, 8, 2, 64, 330
+    x, w, kc, vc, pos, c, s, par = tree_case(B, N, 512, nh, nkv, hd, S, [250, 130, 40], 180 + N, "tree", positions)
+    w["wo"] = (1e-37 * np.eye(512)).astype(np.float32)
+    ramp = np.linspace(0.02, 1.0, S, dtype=np.float32)[:, None]
+    kc[:, :S] *= ramp
+    vc[:, :S] *= np.float32(3e37)
+    vc[1, :S] = np.float32(3.4e38) * np.sign(vc[1, :S])
+    print(f"[gpu-test] values near the largest N={N}", flush=True)
+    got = run_tree(x, w, kc, vc, pos, c, s, par, nh, nkv, hd)
+    y, _, _, live = to.attend(x, (w["wq"], w["wk"], w["wv"], w["wo"]), w["rms"], EPS, c, s, par, pos, kc, vc, nh, nkv, hd)
+    assert live.all() and np.isfinite(got[0]).all()
+    for b in range(B):
+        assert orc.rel_l2(got[0][b].astype(np.float64) - x[b], y[b] - x[b]) <= 1e-5, b
